@@ -1,4 +1,4 @@
-"""ctypes bindings of the two in-tree C-ABI libraries (declared in include/*.h).
+"""ctypes bindings of the three in-tree C-ABI libraries (declared in include/*.h).
 
 The product path has no fallback: if a library is missing or does not load, the ops raise.
 Prototypes here are the ones the reference's own Python binds (r4d_mxfp4_moe.py.lru.diff
@@ -69,7 +69,16 @@ LMHEAD_PROTOS = {
     "b200_moe_gemm_error": (c_int, [c_int]),
 }
 
-LIB_FILES = {"librlu.so": RLU_PROTOS, "libb200lmhead.so": LMHEAD_PROTOS}
+_FP8_OPERANDS = [c_vp, c_ll, c_vp, c_ll, c_ll, c_vp, c_ll, c_int, c_vp, c_ll]
+SCORE_PROTOS = {
+    "b200_fp8_block_gemm": (c_int, _FP8_OPERANDS + [c_vp, c_ll, c_int] + [c_int] * 3 + [c_vp]),
+    "b200_token_logprobs": (c_int, [c_vp, c_int, c_ll, c_int, c_int, c_vp, c_int] + [c_vp] * 6 + [c_vp]),
+    "b200_fp8_head_logprobs_workspace_bytes": (c_ll, [c_int, c_int]),
+    "b200_fp8_head_logprobs": (c_int, _FP8_OPERANDS + [c_vp] + [c_int] * 3 + [c_vp] * 4 + [c_ll, c_vp]),
+    "b200_score_error": (c_int, [c_int]),
+}
+
+LIB_FILES = {"librlu.so": RLU_PROTOS, "libb200lmhead.so": LMHEAD_PROTOS, "libb200score.so": SCORE_PROTOS}
 
 
 class NativeLibraryError(RuntimeError):
@@ -77,7 +86,8 @@ class NativeLibraryError(RuntimeError):
 
 
 def lib_path(name: str) -> str:
-    env = {"librlu.so": "R4D_LRU_LIB", "libb200lmhead.so": "B200_LMHEAD_LIB"}[name]
+    env = {"librlu.so": "R4D_LRU_LIB", "libb200lmhead.so": "B200_LMHEAD_LIB",
+           "libb200score.so": "B200_SCORE_LIB"}[name]
     return os.environ.get(env) or os.path.join(HERE, name)
 
 
@@ -110,6 +120,10 @@ def lmhead() -> ctypes.CDLL:
     return load("libb200lmhead.so")
 
 
+def score() -> ctypes.CDLL:
+    return load("libb200score.so")
+
+
 def ptr(t) -> c_vp:
     return c_vp(0 if t is None else t.data_ptr())
 
@@ -140,6 +154,18 @@ def debug_check(what: str) -> None:
     if err != 0:
         raise RuntimeError(f"{what}: device error word {err} (1: a pipeline wait ran out, "
                            "2: a peer's statistics did not arrive); clear it with b200_lmhead_error(1)")
+
+
+def debug_check_score(what: str) -> None:
+    """debug_check for the scoring kernels' own error word."""
+    if not _CHECK:
+        return
+    import torch
+    torch.cuda.current_stream().synchronize()
+    err = int(score().b200_score_error(0))
+    if err != 0:
+        raise RuntimeError(f"{what}: device error word {err} (1: a pipeline wait ran out); "
+                           "clear it with b200_score_error(1)")
 
 
 def require_cuda(what: str, *tensors) -> None:

@@ -1,16 +1,19 @@
-"""Build the two C-ABI shared libraries of this package, in-tree, for sm_100a.
+"""Build the three C-ABI shared libraries of this package, in-tree, for sm_100a.
 
 * ``librlu.so``       -- csrc/lru.cu: r4d_lru_manage / r4d_lru_fused / r4d_lru_gather.
 * ``libb200lmhead.so`` -- csrc/quant.cu + csrc/lmhead.cu + csrc/gate.cu + csrc/moe_sum.cu +
   csrc/moe_gemm.cu: SiLU-mul FP8 quant, per-token (group) FP8 quant, FP8 and W4 lm_head
   GEMVs, the stream control, the shared-expert gate, the routed experts' sum and the grouped
   MXFP4 x FP8 MoE GEMM.
+* ``libb200score.so`` -- csrc/fp8_gemm.cu + csrc/logprobs.cu: the FP8 block-scaled product for any
+  number of tokens, token log probabilities, the FP8 head straight to log probabilities.
 
 No fast math: the SiLU-quant parity needs IEEE division and the accurate expf.
 Usage: ``python build.py [--force]`` (also called by ``__graft_entry__.build()``).
 """
 from __future__ import annotations
 
+import glob
 import os
 import shutil
 import subprocess
@@ -25,6 +28,7 @@ FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
 LIBS = {
     "librlu.so": ["lru.cu"],
     "libb200lmhead.so": ["quant.cu", "lmhead.cu", "gate.cu", "moe_sum.cu", "moe_gemm.cu"],
+    "libb200score.so": ["fp8_gemm.cu", "logprobs.cu"],
 }
 
 
@@ -39,7 +43,7 @@ def _stale(out: str, srcs: list[str]) -> bool:
     if not os.path.exists(out):
         return True
     t = os.path.getmtime(out)
-    deps = srcs + [os.path.join(CSRC, "common.cuh"), os.path.abspath(__file__)]
+    deps = srcs + glob.glob(os.path.join(CSRC, "*.cuh")) + [os.path.abspath(__file__)]
     return any(os.path.getmtime(d) > t for d in deps)
 
 

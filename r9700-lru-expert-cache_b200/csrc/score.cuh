@@ -1,0 +1,52 @@
+// Shared pieces of the scoring kernels (fp8_gemm.cu, logprobs.cu).
+#pragma once
+#include "common.cuh"
+
+namespace b200 {
+
+// Statistics of a row of logits relative to a reference m (its running maximum):
+// s = sum e^(x - m), w = sum e^(x - m) (x - m). m = -inf: nothing but -inf so far, s = w = 0.
+struct LogitStat {
+  float m, s, w;
+};
+
+B200_DEVINL LogitStat logit_stat_empty() { return LogitStat{-INFINITY, 0.f, 0.f}; }
+
+// Merge in either order. Moving a part from its m to the larger M, with t = m - M <= 0:
+// e^(x - M) = e^(x - m) e^t and x - M = (x - m) + t. A part with m = -inf contributes nothing
+// (its t would be NaN or -inf, times zero); a NaN in s passes through.
+B200_DEVINL LogitStat logit_stat_merge(const LogitStat& a, const LogitStat& b) {
+  LogitStat o;
+  o.m = fmaxf(a.m, b.m);
+  const float ta = a.m == -INFINITY ? 0.f : a.m - o.m, tb = b.m == -INFINITY ? 0.f : b.m - o.m;
+  const float ea = expf(ta), eb = expf(tb);
+  // where e^t is 0 (t may be -inf) the part is below fp32's reach: s e^t = 0 and so is its w
+  const float wa = ea > 0.f ? (a.w + a.s * ta) * ea : 0.f, wb = eb > 0.f ? (b.w + b.s * tb) * eb : 0.f;
+  o.s = a.s * ea + b.s * eb;
+  o.w = wa + wb;
+  return o;
+}
+
+struct RowResult {
+  float logprob, entropy, lse;
+};
+
+// xt: the token's logit; valid: its id is inside the vocabulary.
+B200_DEVINL RowResult logit_stat_finish(const LogitStat& st, float xt, bool valid) {
+  RowResult r;
+  if (st.m == -INFINITY && !isnan(st.s)) {
+    r.lse = -INFINITY;
+    r.entropy = 0.f;
+    r.logprob = -INFINITY;
+  } else {
+    const float ls = logf(st.s);
+    r.lse = st.m + ls;
+    r.entropy = ls - st.w / st.s;
+    r.logprob = (xt - st.m) - ls;
+  }
+  if (isnan(st.s)) r.lse = r.entropy = r.logprob = NAN;
+  if (!valid) r.logprob = NAN;
+  return r;
+}
+
+}  // namespace b200

@@ -1,0 +1,81 @@
+"""``fp8_block_gemm``: the FP8 128x128 block-scaled matrix product for any number of tokens, backed
+by the sm_100a kernels of csrc/fp8_gemm.cu (``b200_fp8_block_gemm``).
+
+The FP8 target head (``fp8_target_lmhead``) passes over its weight once for 64 tokens; a prompt's
+hundreds or thousands of rows go through this product instead, with the same operands: activations
+e4m3 with an fp32 scale for each row's group of 128 (``per_token_group_quant_fp8``,
+``silu_mul_quant_group``) and weights e4m3 with an fp32 scale for each block of 128 x 128, row-major
+as a checkpoint holds them or in the head's strip pack (``pack_fp8_block``).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_BLK = 128
+FP8 = torch.float8_e4m3fn
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _operands(what: str, qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: torch.Tensor,
+              packed: bool) -> tuple:
+    """Checks the four operands and returns the C entries' leading arguments with M, N and K."""
+    _lib.require_cuda(what, qx, wq, xs, ws)
+    if qx.ndim != 2 or wq.ndim != 2 or qx.dtype != FP8 or wq.dtype != FP8:
+        raise ValueError(f"{what}: qx and wq must be 2-D e4m3 tensors")
+    (M, K), N = qx.shape, wq.shape[0]
+    if wq.shape[1] != K:
+        raise ValueError(f"{what}: weight {tuple(wq.shape)} does not match activations {tuple(qx.shape)}")
+    if N < 1 or K < 16 or K % 16:
+        raise ValueError(f"{what}: N must be at least 1 and K a positive multiple of 16 (N={N}, K={K})")
+    kb, nb = -(-K // _BLK), -(-N // _BLK)
+    if xs.dtype != torch.float32 or xs.shape != (M, kb):
+        raise ValueError(f"{what}: xs must be fp32 [{M}, {kb}], got {xs.dtype} {tuple(xs.shape)}")
+    if ws.dtype != torch.float32 or ws.shape != (nb, kb) or (kb > 1 and ws.stride(1) != 1):
+        raise ValueError(f"{what}: ws must be fp32 [{nb}, {kb}] with unit column stride, got {ws.dtype} "
+                         f"{tuple(ws.shape)}")
+    if len({t.device for t in (qx, wq, xs, ws)}) != 1:
+        raise ValueError(f"{what}: operands are on different devices")
+    if packed:
+        if N % 16 or K % _BLK or not wq.is_contiguous():
+            raise ValueError(f"{what}: a strip pack is contiguous with N % 16 == 0 and K % 128 == 0")
+    ldx = qx.stride(0) if M > 1 else K
+    ldw = wq.stride(0) if N > 1 else K
+    if qx.stride(1) != 1 or (not packed and wq.stride(1) != 1) or ldx < K or ldw < K or ldx % 16 or ldw % 16:
+        raise ValueError(f"{what}: rows of qx and wq must be contiguous, their strides multiples of 16")
+    if (M and qx.data_ptr() % 16) or wq.data_ptr() % 16:
+        raise ValueError(f"{what}: qx and wq must be 16-byte aligned")
+    args = (qx.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), wq.data_ptr(), ldw, int(packed),
+            ws.data_ptr(), ws.stride(0))
+    return args, M, N, K
+
+
+def fp8_block_gemm(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: torch.Tensor,
+                   out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None,
+                   packed: bool = False) -> torch.Tensor:
+    """(qx * xs) @ (wq * ws).T -> [M, N] in ``out_dtype`` (bf16, f16 or f32) or into ``out``.
+
+    qx e4m3 [M, K], xs fp32 [M, ceil(K/128)] (any strides, so a group-major scale tensor may be
+    passed transposed), wq e4m3 [N, K] row-major (or, with ``packed``, the strip pack of
+    ``pack_fp8_block``), ws fp32 [ceil(N/128), ceil(K/128)]. K is a multiple of 16; rows of qx and
+    wq may be strided by multiples of 16. Each 128-K block's sum is scaled and added in fp32 and
+    the result rounded once."""
+    args, M, N, K = _operands("fp8_block_gemm", qx, wq, xs, ws, packed)
+    if out is None:
+        if out_dtype not in _DTYPES:
+            raise ValueError(f"fp8_block_gemm: unsupported output dtype {out_dtype}")
+        out = torch.empty(M, N, dtype=out_dtype, device=qx.device)
+    else:
+        _lib.require_cuda("fp8_block_gemm", out)
+        if out.shape != (M, N) or out.dtype not in _DTYPES or out.device != qx.device or \
+                (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError(f"fp8_block_gemm: out must be bf16, f16 or f32 [{M}, {N}] on {qx.device} with unit "
+                             "column stride and rows that do not overlap")
+    if M:
+        with torch.cuda.device(qx.device):
+            rc = _lib.score().b200_fp8_block_gemm(*args, out.data_ptr(), out.stride(0) if M > 1 else N,
+                                                  _DTYPES[out.dtype], M, N, K, _lib.stream_ptr())
+            _lib.check(rc, "b200_fp8_block_gemm")
+            _lib.debug_check_score("b200_fp8_block_gemm")
+    return out
