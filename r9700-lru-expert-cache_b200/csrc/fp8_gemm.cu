@@ -1,6 +1,23 @@
 // FP8 128x128 block-scaled matrix product for any number of tokens, and the same product reduced
 // to the log probabilities of given tokens.
+//
+//   y[m, n] = sum_b xs[m, b] ws[n / 128, b] D_b[m, n],   D_b[m, n] = sum_{k in block b} qx[m, k] wq[n, k]
+//
+// Each D_b is one accumulator of the tensor core (fp32, TMEM): 128 tokens x BN weight rows, 128 K. The
+// weight's scale is one number over the tile's 128 rows and the token's is one number per TMEM lane, so a
+// thread that holds a lane's columns needs ONE factor per block: the promotion of D_b into the running sum is
+// a tcgen05.ld and one fused multiply-add per value, in registers, while the MMAs fill the other accumulators.
+//   warp 0     one lane copies the tiles (tensor maps: zeros beyond M, N and K) into a ring of stages;
+//   warp 1     one lane issues the MMAs, four of K = 32 a stage, a fresh accumulator for every 128-K block;
+//   warp 2     puts the factors xs ws of four 128-K blocks at a time into shared memory;
+//   warps 4-11 two groups of four, each with half of the columns: promote, then write the tile.
+// CTAs (or pairs) walk the tiles, rows first within groups of row tiles, so that tiles in flight share weights.
+#include <algorithm>
+
+#include <cudaTypedefs.h>
+
 #include "score.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -8,123 +25,507 @@ using namespace b200;
 
 __device__ int g_score_err = 0;
 
-struct Operands {
-  const uint8_t* x;
-  long long ldx;
+constexpr int EPI_GROUPS = 2, EPI_WARPS = 4 * EPI_GROUPS;
+constexpr int THREADS = 32 * (4 + EPI_WARPS);
+constexpr int BM = 128;                    // token rows of a CTA's tile (TMEM lanes)
+constexpr int SMEM_CAP = 227 * 1024;
+constexpr int MAX_STAGES = 12;
+// Every CTA takes all of TMEM, so no two may share an SM (a second one's allocation would wait, and CTAs of
+// two clusters could wait for each other): each asks for more than half of the shared memory.
+constexpr int SMEM_MIN = 116 * 1024;
+constexpr int FGROUP = 4;                  // 128-K blocks whose factors are written at a time
+constexpr int F_LD = 2 * BM + 8;           // of one block: [column block][row], padded against bank conflicts
+constexpr int GROUP_ROWS = 16;             // row tiles that share a stretch of the weight
+
+struct Product {
   const float* xs;
   long long xs_row, xs_col;
-  const uint8_t* w;
-  long long ldw;
-  int packed;
   const float* ws;
   long long ws_row;
   int M, N, K;
+  int packed;
+  int box_m;                               // token rows that a stage's copy brings
+  int row_tiles, col_tiles;
+  int nstage;
+  // op 1
+  void* y;
+  long long ldy;
+  int tma_out;                             // y's base and rows are 16-byte aligned
+  // head: part [column group][3][M], token [M]
+  const long long* ids;
+  float* part;
+  float* token;
 };
 
-// Byte of weight element (n, k): row-major, or the strip pack [N/16][K/128][16 rows][128 B] with
-// 16-byte chunk c of strip row r at chunk c ^ (r & 7).
-__device__ __forceinline__ long long weight_at(const Operands& p, int n, int k) {
-  if (!p.packed) return n * p.ldw + k;
-  const int r = n & 15, c = (k & 127) >> 4;
-  return ((long long)(n >> 4) * (p.K >> 7) + (k >> 7)) * 2048 + r * 128 + ((c ^ (r & 7)) << 4) + (k & 15);
+enum Out { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2, OUT_STATS = 3 };
+
+// How a tile's 128-K block goes through TMEM. BN <= 128: one accumulator of BN columns, half of it for each
+// epilogue group. BN = 256: two accumulators of 128 columns, one for each group, with barriers of their own, so
+// that four are in flight: an accumulator's way from its last MMA through commit, load and release back to its
+// next MMA takes longer than the other one's MMAs.
+template <int BN>
+struct Tile {
+    static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
+  static constexpr int UN = BN / UNITS;             // their columns
+  static constexpr int W = BN / EPI_GROUPS;         // columns of one epilogue group
+  static constexpr int CHUNK = W < 32 ? W : 32;     // columns of one TMEM load
+  static constexpr int NBUF = 512 / UN > 8 ? 8 : 512 / UN;
+  static constexpr int RELEASERS = UNITS == 2 ? EPI_WARPS / 2 : EPI_WARPS;   // warps of a CTA that read one
+  static constexpr int BLOCKS = BN > 128 ? BN / 128 : 1;   // weight scales of a tile's 128-K block
+  // Register split of the launch's 168 registers a thread: the running sums of BN = 256 need more.
+  static constexpr bool SPLIT_REGS = BN == 256;
+  static constexpr int LAUNCH_REGS = 168, EPI_REGS = 216, OTHER_REGS = 72;
+  static_assert(EPI_REGS * EPI_WARPS + OTHER_REGS * 4 <= LAUNCH_REGS * (EPI_WARPS + 4), "more than the launch brings");
+};
+
+// Tile number -> (row tile, column tile).
+__device__ __forceinline__ void tile_at(const Product& p, int t, int& rt, int& ct) {
+  const int per_group = GROUP_ROWS * p.col_tiles, g = t / per_group, r = t - g * per_group;
+  const int rows = min(GROUP_ROWS, p.row_tiles - g * GROUP_ROWS);
+  ct = r / rows;
+  rt = g * GROUP_ROWS + (r - ct * rows);
 }
 
-__device__ __forceinline__ float e4m3_to_f32(uint8_t b) {
-  __nv_fp8_e4m3 v;
-  v.__x = b;
-  return float(v);
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-template <>
-__device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+// Column c of a group's W, counted from the group's first one.
+template <bool SEG>
+__host__ __device__ __forceinline__ constexpr int column(int c) {
+  return SEG && c >= 64 ? c + 64 : c;
+}
 
-constexpr int T = 64;
+template <int OUT>
+__device__ __forceinline__ void store_one(void* row, int col, float v) {
+  if (OUT == OUT_BF16) static_cast<__nv_bfloat16*>(row)[col] = __float2bfloat16_rn(v);
+  if (OUT == OUT_F16) static_cast<__half*>(row)[col] = __float2half_rn(v);
+  if (OUT == OUT_F32) static_cast<float*>(row)[col] = v;
+}
 
-// One 64 x 64 tile of y per CTA, 256 threads of 4 x 4 outputs, K in steps of 16.
-__device__ __forceinline__ void product_tile(const Operands& p, int m0, int n0, float (&acc)[4][4]) {
-  __shared__ float xa[16][T + 1], wa[16][T + 1];
-  const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  float part[4][4] = {};
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    for (int e = threadIdx.x; e < 16 * T; e += 256) {
-      const int r = e >> 4, k = e & 15;
-      xa[k][r] = m0 + r < p.M ? e4m3_to_f32(p.x[(m0 + r) * p.ldx + k0 + k]) : 0.f;
-      wa[k][r] = n0 + r < p.N ? e4m3_to_f32(p.w[weight_at(p, n0 + r, k0 + k)]) : 0.f;
+// Writes a warp's 32 rows x W columns of y at (m0, n0), 64 bytes a row at a time through one of two 2 KB
+// buffers: a tensor-map store that runs on while the warp goes back to its next tile (rows beyond M and columns
+// beyond N are clipped by the copy), or, where y's base or rows are not 16-byte aligned, plain coalesced stores.
+// Straight from registers, 32 rows an instruction, the same tile took 6400 clocks of the 10240 that its MMAs
+// take at K = 2560.
+template <int OUT, int W, bool SEG>
+__device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* ymap, char* bufs, int& turn, int m0,
+                                           int n0, int lane, const float2 (&acc)[W / 2]) {
+  constexpr int ES = OUT == OUT_F32 ? 4 : 2, CC = 64 / ES;
+#pragma unroll
+  for (int c = 0; c < W; c += CC, ++turn) {
+    char* buf = bufs + (turn & 1) * 2048;
+    const int n = n0 + column<SEG>(c);
+    if (lane == 0) bulk_wait_read<1>();              // this buffer's last store has been read
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (OUT == OUT_F32) v[i] = __float_as_uint(i & 1 ? acc[(c + 4 * q + i) / 2].y : acc[(c + 4 * q + i) / 2].x);
+        if (OUT == OUT_BF16) v[i] = pack_bf16(acc[c / 2 + 4 * q + i].x, acc[c / 2 + 4 * q + i].y);
+        if (OUT == OUT_F16) v[i] = pack_f16(acc[c / 2 + 4 * q + i].x, acc[c / 2 + 4 * q + i].y);
+      }
+      // 64-byte swizzle: 16-byte piece q of row r at piece q ^ ((r / 2) mod 4)
+      *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
     }
-    __syncthreads();
-    for (int k = 0; k < 16; ++k)
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) part[i][j] = fmaf(xa[k][ty * 4 + i], wa[k][tx * 4 + j], part[i][j]);
-    __syncthreads();
-    if ((k0 & 127) == 112 || k0 + 16 >= p.K) {
-      const int b = k0 >> 7;
-      for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-          const int m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-          const float s = m < p.M && n < p.N ? p.xs[m * p.xs_row + b * p.xs_col] * p.ws[(n >> 7) * p.ws_row + b] : 0.f;
-          acc[i][j] = fmaf(part[i][j], s, acc[i][j]);
-          part[i][j] = 0.f;
+    if (p.tma_out) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (n < p.N) tma_store_2d(ymap, n, m0, smem_u32(buf));
+        bulk_commit();
+      }
+    } else {
+      __syncwarp();
+      char* y = static_cast<char*>(p.y);
+#pragma unroll 4
+      for (int i = lane; i < 32 * CC; i += 32) {
+        const int r = i / CC, col = i % CC;
+        if (m0 + r < p.M && n + col < p.N) {
+          const char* from = buf + r * 64 + (((col * ES >> 4) ^ ((r >> 1) & 3)) << 4) + (col * ES & 15);
+          char* to = y + ((long long)(m0 + r) * p.ldy + n + col) * ES;
+          if (ES == 4)
+            *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
+          else
+            *reinterpret_cast<uint16_t*>(to) = *reinterpret_cast<const uint16_t*>(from);
         }
+      }
+      __syncwarp();
     }
   }
 }
 
-template <typename OUT>
-__global__ void __launch_bounds__(256) gemm_kernel(Operands p, OUT* y, long long ldy) {
-  float acc[4][4];
-  const int m0 = blockIdx.y * T, n0 = blockIdx.x * T;
-  product_tile(p, m0, n0, acc);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + (threadIdx.x >> 4) * 4 + i, n = n0 + (threadIdx.x & 15) * 4 + j;
-      if (m < p.M && n < p.N) y[m * ldy + n] = from_f32<OUT>(acc[i][j]);
+// A row's statistics over the W values of a group whose first column is n, and its token's logit if it is one.
+template <int W, bool SEG>
+__device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, const float2 (&acc)[W / 2]) {
+  auto at = [&](int c) { return c & 1 ? acc[c / 2].y : acc[c / 2].x; };
+  auto in = [&](int c) { return n + column<SEG>(c) < p.N; };
+  const long long id = p.ids[m] - n;
+  if (id >= 0 && id < column<SEG>(W - 1) + 1 && id < p.N - n) {
+    float v = NAN;
+    bool mine = false;
+#pragma unroll
+    for (int c = 0; c < W; ++c)
+      if (column<SEG>(c) == (int)id) v = at(c), mine = true;
+    if (mine) p.token[m] = v;
+  }
+  LogitStat st;
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  float odd[4] = {};                                 // NaN once a NaN or an infinity of either sign was seen
+#pragma unroll
+  for (int c = 0; c < W; ++c)
+    if (in(c)) {
+      mx[c & 3] = fmaxf(mx[c & 3], at(c));
+      odd[c & 3] = fmaf(at(c), 0.f, odd[c & 3]);
     }
+  st.m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  float s[4] = {}, w[4] = {};
+#pragma unroll
+  for (int c = 0; c < W; ++c) {
+    const float d = in(c) ? fmaxf(at(c) - st.m, -200.f) : -200.f;  // e^-200 = 0 in fp32, and 0 * -200 = 0
+    const float e = __expf(d);
+    s[c & 3] += e;
+    w[c & 3] = fmaf(e, d, w[c & 3]);
+  }
+  st.s = (s[0] + s[1]) + (s[2] + s[3]);
+  st.w = (w[0] + w[1]) + (w[2] + w[3]);
+  if (st.m == -INFINITY) st.s = st.w = 0.f;
+  if (isnan((odd[0] + odd[1]) + (odd[2] + odd[3]))) {
+    // -inf beside finite values is as if it were absent; NaN and +inf make the row NaN
+    bool nan = st.m == INFINITY;
+#pragma unroll
+    for (int c = 0; c < W; ++c) nan |= in(c) && isnan(at(c));
+    if (nan) st = LogitStat{0.f, NAN, NAN};
+  }
+  return st;
 }
 
-// part [column tile][3][M]; token [M]
-__global__ void __launch_bounds__(256)
-    head_kernel(Operands p, const long long* __restrict__ ids, float* __restrict__ part, float* __restrict__ token) {
-  __shared__ float tile[T][T + 1];
-  float acc[4][4];
-  const int m0 = blockIdx.y * T, n0 = blockIdx.x * T;
-  product_tile(p, m0, n0, acc);
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) tile[(threadIdx.x >> 4) * 4 + i][(threadIdx.x & 15) * 4 + j] = acc[i][j];
+// Shared memory: barriers | factors [2][FGROUP][F_LD] | output buffers or statistics | ring of stages.
+__host__ __device__ constexpr int out_offset() { return (1024 + 2 * FGROUP * F_LD * 4 + 1023) / 1024 * 1024; }
+template <int OUT>
+__host__ __device__ constexpr int ring_offset() {
+  return out_offset() + (OUT == OUT_STATS ? 2 * 3 * EPI_GROUPS * BM * 4 : EPI_WARPS * 4096);
+}
+
+// One CTA (CG = 1; gridDim / cluster size clusters, whose CTAs split K) or one CTA pair (CG = 2).
+template <int CG, int BN, int OUT>
+__global__ void __launch_bounds__(THREADS, 1)
+    product_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+                   const __grid_constant__ CUtensorMap ymap, Product p) {
+  constexpr int W = Tile<BN>::W, NBUF = Tile<BN>::NBUF, UNITS = Tile<BN>::UNITS, UN = Tile<BN>::UN;
+  constexpr bool SEG = CG == 2 && UNITS == 2;                      // a group's columns: 64 of each 128-column block
+  constexpr int B_ROWS = BN / CG;                    // weight rows in this CTA's shared memory
+  constexpr int STAGE = (BM + B_ROWS) * 128;
+  constexpr bool CAN_SPLIT = CG == 1 && OUT != OUT_STATS && !Tile<BN>::SPLIT_REGS;
+  extern __shared__ char sm_raw[];
+  char* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sm);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* acc_full = empty + MAX_STAGES;
+  uint64_t* acc_empty = acc_full + 8;
+  uint64_t* f_full = acc_empty + 8;
+  uint64_t* f_empty = f_full + 2;
+  uint64_t* done = f_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  float* factors = reinterpret_cast<float*>(sm + 1024);
+  float* stat_s = reinterpret_cast<float*>(sm + out_offset());      // head: [2][3][EPI_GROUPS][BM]
+  char* ring = sm + ring_offset<OUT>();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_rank(), csize = cluster_size();
+  const uint32_t split = CAN_SPLIT ? csize : 1, part = CAN_SPLIT ? crank : 0;
+  const int KB = (p.K + 127) >> 7;
+  const int kb0 = KB * part / split, kb1 = KB * (part + 1) / split;
+  const int tiles = p.row_tiles * p.col_tiles;
+  const int first = blockIdx.x / csize, step = gridDim.x / csize;
+  const int nstage = p.nstage;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < nstage; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], UNITS);
+    }
+    for (int i = 0; i < NBUF; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], Tile<BN>::RELEASERS * CG);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&f_full[i], 1);
+      mbar_init(&f_empty[i], EPI_WARPS);
+    }
+    mbar_init(done, UNITS);
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_512<CG>(tmem_slot);
+  tc_fence_before();
   __syncthreads();
-  const int m = m0 + threadIdx.x;
-  if (threadIdx.x < T && m < p.M) {
-    LogitStat st = logit_stat_empty();
-    const long long id = ids[m];
-    for (int j = 0; j < T && n0 + j < p.N; ++j) {
-      const float f = tile[threadIdx.x][j];
-      if (n0 + j == id) token[m] = f;
-      LogitStat one = {f, f == -INFINITY ? 0.f : 1.f, 0.f};
-      if (isnan(f) || f == INFINITY) one = LogitStat{0.f, NAN, NAN};
-      st = logit_stat_merge(st, one);
+  if (csize > 1) cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  float2 acc[W / 2];
+  if (Tile<BN>::SPLIT_REGS && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Tile<BN>::OTHER_REGS));
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- copies ----------------
+      const uint32_t rank = CG == 2 ? crank : 0;
+      const uint32_t bytes = (p.box_m + B_ROWS) * 128 * CG;
+      int it = 0, s = 0, round = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        int rt, ct;
+        tile_at(p, t, rt, ct);
+        const int m = (rt * CG + (int)rank) * BM, n = ct * BN + (int)rank * B_ROWS;
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          if (round > 0 && !mbar_wait_limited(&empty[s], (round - 1) & 1)) {
+            ok = false;
+            break;
+          }
+          uint32_t bar = smem_u32(&full[s]);
+          if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+          if (CG == 2) bar = map_to_rank(bar, 0);
+          const uint32_t dst = smem_u32(ring + s * STAGE);
+          tma_load_2d<CG>(dst, &xmap, kb * 128, m, bar);
+          if (p.packed)
+            tma_load_4d<CG>(dst + BM * 128, &wmap, 0, 0, n / 16, kb, bar);
+          else
+            tma_load_2d<CG>(dst + BM * 128, &wmap, kb * 128, n, bar);
+          if (++s == nstage) s = 0, ++round;
+        }
+      }
+      // Leave only when this CTA's copies have landed and been read: the MMAs' commit of each stage's last use.
+      const int last = min(it, nstage);
+      for (int i = 0; i < last && ok; ++i) {
+        const int q = it - last + i;
+        ok = mbar_wait_limited(&empty[q % nstage], (q / nstage) & 1);
+      }
+      if (!ok) {
+        atomicExch(&g_score_err, 1);
+        if (CG == 1 || rank == 0)
+          for (int i = 0; i < last; ++i) mbar_wait_limited(&full[(it - last + i) % nstage], ((it - last + i) / nstage) & 1);
+        else                                           // the pair's barriers are the other CTA's: time for any copy to land
+          for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000ull;) __nanosleep(1000);
+      }
     }
-    float* o = part + (long long)blockIdx.x * 3 * p.M + m;
-    o[0] = st.m;
-    o[p.M] = st.s;
-    o[2LL * p.M] = st.w;
+    __syncwarp();
+  } else if (warp == 1 || (UNITS == 2 && warp == 3)) {
+    if (CG == 1 || crank == 0) {
+      // ---------------- MMAs: warp 1 the first accumulator of a block, warp 3 the second one ----------------
+      // The whole warp walks the loop and one elected lane issues.
+      const uint32_t idesc = (1u << 4)                             // D: f32
+                             | ((uint32_t)(UN >> 3) << 17)         // N
+                             | ((uint32_t)(BM * CG >> 4) << 24);   // M; A, B: e4m3, K-major
+      const int u = warp >> 1;
+      int s = 0, round = 0, buf = u, use = 0;
+      bool ok = true;
+      for (int t = first; t < tiles && ok; t += step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          ok = warp_wait(&full[s], round & 1, &acc_empty[buf], (use - 1) & 1, use > 0);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t st = smem_u32(ring + s * STAGE);
+            const uint64_t a = sw128_desc(st), b = sw128_desc(st + BM * 128 + u * (UN / CG * 128));
+            const uint32_t d = tmem + buf * UN;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) tc_mma_f8<CG>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : 0u);
+            tc_commit<CG>(&acc_full[buf]);
+            tc_commit<CG>(&empty[s]);
+          }
+          __syncwarp();
+          if (++s == nstage) s = 0, ++round;
+          buf += UNITS;
+          if (buf >= NBUF) buf -= NBUF, ++use;
+        }
+      }
+      if (!ok) {                                       // what was issued still writes TMEM
+        if (elect_one()) {
+          atomicExch(&g_score_err, 1);
+          tc_commit<CG>(done);
+        }
+        __syncwarp();
+        mbar_wait_limited(done, 0);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ---------------- factors ----------------
+    // Lane = (row mod 8, block of the group): row-major scales are read 16 B a row, four blocks in one pass.
+    const int r8 = lane >> 2, i = lane & 3;
+    const uint32_t rank = CG == 2 ? crank : 0;
+    int fg = 0;
+    bool ok = true;
+    for (int t = first; t < tiles && ok; t += step) {
+      int rt, ct;
+      tile_at(p, t, rt, ct);
+      const int m = (rt * CG + (int)rank) * BM + r8, nb = ct * BN >> 7;
+      for (int kb = kb0; kb < kb1; kb += FGROUP, ++fg) {
+        float x[BM / 8], w[Tile<BN>::BLOCKS];
+#pragma unroll
+        for (int b = 0; b < Tile<BN>::BLOCKS; ++b)
+          w[b] = kb + i < kb1 && (nb + b) * 128 < p.N ? __ldg(p.ws + (long long)(nb + b) * p.ws_row + kb + i) : 0.f;
+#pragma unroll
+        for (int j = 0; j < BM / 8; ++j)
+          x[j] = kb + i < kb1 && m + 8 * j < p.M
+                     ? __ldg(p.xs + (long long)(m + 8 * j) * p.xs_row + (long long)(kb + i) * p.xs_col) : 0.f;
+        if (fg >= 2) ok = warp_wait(&f_empty[fg & 1], ((fg >> 1) - 1) & 1);
+        if (!ok) break;
+        float* dst = factors + ((fg & 1) * FGROUP + i) * F_LD + r8;
+#pragma unroll
+        for (int b = 0; b < Tile<BN>::BLOCKS; ++b)
+#pragma unroll
+          for (int j = 0; j < BM / 8; ++j) dst[b * BM + 8 * j] = x[j] * w[b];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&f_full[fg & 1]);
+      }
+    }
+    if (!ok && lane == 0) atomicExch(&g_score_err, 1);
+  } else if (warp >= 4) {
+    // ---------------- promotion and output ----------------
+    if constexpr (Tile<BN>::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Tile<BN>::EPI_REGS));
+    const int quarter = warp & 3, group = (warp >> 2) - 1;
+    const uint32_t rank = CG == 2 ? crank : 0;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + (UNITS == 1 ? group * W : 0);
+    const int row_in_tile = 32 * quarter + lane;
+    const float* my_factors = factors + (BN == 256 && !SEG ? group : 0) * BM + row_in_tile;
+    const int col = SEG ? 64 * group : W * group;    // first column of the group in its tile
+    int buf = UNITS == 2 ? group : 0, use = 0, turn = 0, fg = 0;
+    bool ok = true;
+    for (int t = first; t < tiles; t += step) {
+      int rt, ct;
+      tile_at(p, t, rt, ct);
+      const int m = (rt * CG + (int)rank) * BM + row_in_tile, n = ct * BN + col;
+#pragma unroll
+      for (int c = 0; c < W / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        const int fi = (kb - kb0) & (FGROUP - 1);
+        ok = warp_wait(&acc_full[buf], use & 1, &f_full[fg & 1], (fg >> 1) & 1, fi == 0);
+        if (!ok) break;
+        tc_fence_after();
+        const float* now = my_factors + ((fg & 1) * FGROUP + fi) * F_LD;
+        const float scale0 = now[0], scale1 = SEG ? now[BM] : scale0;
+        const uint32_t src = lanes + buf * UN;
+        constexpr int C = Tile<BN>::CHUNK;
+        uint32_t v[2][C];
+        tmem_ld<C>(src, v[0]);
+#pragma unroll
+        for (int c = 0; c < W; c += C) {
+          uint32_t(&x)[C] = v[c / C & 1];
+          tmem_wait_ld<C>(x);
+          if (c + C < W) {
+            tmem_ld<C>(src + c + C, v[(c / C & 1) ^ 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if (CG == 1 || rank == 0)
+                mbar_arrive(&acc_empty[buf]);
+              else
+                mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < C / 2; ++i) fma2_scaled(acc[c / 2 + i], x[2 * i], x[2 * i + 1], c < 64 ? scale0 : scale1);
+        }
+        if (fi == FGROUP - 1 || kb + 1 == kb1) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&f_empty[fg & 1]);
+          ++fg;
+        }
+        buf += UNITS;
+        if (buf >= NBUF) buf -= NBUF, ++use;
+      }
+      if constexpr (OUT == OUT_STATS) {
+        // a tile's four column groups leave one set of statistics
+        float* own = stat_s + (turn & 1) * 3 * EPI_GROUPS * BM + row_in_tile;
+        LogitStat st = logit_stat_empty();
+        if (ok && m < p.M && n < p.N) st = row_stats<W, SEG>(p, m, n, acc);
+        own[(0 * EPI_GROUPS + group) * BM] = st.m;
+        own[(1 * EPI_GROUPS + group) * BM] = st.s;
+        own[(2 * EPI_GROUPS + group) * BM] = st.w;
+        asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+        if (group == 0 && m < p.M) {
+#pragma unroll
+          for (int g = 1; g < EPI_GROUPS; ++g)
+            st = logit_stat_merge(st, LogitStat{own[g * BM], own[(EPI_GROUPS + g) * BM], own[(2 * EPI_GROUPS + g) * BM]});
+          float* o = p.part + (long long)ct * 3 * p.M + m;
+          o[0] = st.m;
+          o[p.M] = st.s;
+          o[2LL * p.M] = st.w;
+        }
+        ++turn;
+      } else if (ok && split == 1 && n < p.N && m - lane < p.M) {
+        store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (warp - 4) * 4096, turn, m - lane, n, lane, acc);
+      }
+    }
+    if (OUT != OUT_STATS && lane == 0) bulk_wait_all();
+    if (!ok && lane == 0) atomicExch(&g_score_err, 1);
   }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CAN_SPLIT) {
+    // ---------------- K split over the cluster's CTAs: one tile, whose ring is idle now ----------------
+    if (split > 1) {
+      constexpr int LD = BN + 4;
+      float* sums = reinterpret_cast<float*>(ring);
+      int rt, ct;
+      tile_at(p, first, rt, ct);
+      const int rows = min(BM, p.M - rt * BM);
+      if (warp >= 4) {
+        const int group = (warp >> 2) - 1, r = 32 * (warp & 3) + lane;
+        if (r < rows) {
+#pragma unroll
+          for (int c = 0; c < W; c += 4)
+            *reinterpret_cast<float4*>(sums + r * LD + group * W + c) =
+                make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y);
+        }
+      }
+      cluster_sync_all();
+      // each CTA adds, in rank order, its share of the columns
+      const int share = BN / split, quads = share / 4;
+      const uint32_t mine = smem_u32(sums);
+      for (int e = threadIdx.x; e < rows * quads; e += THREADS) {
+        const int r = e / quads, c = part * share + (e - r * quads) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (uint32_t q = 0; q < split; ++q) {
+          const float4 u = ld_cluster_f4(map_to_rank(mine + (r * LD + c) * 4, q));
+          v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+        }
+        const int n = ct * BN + c;
+        char* at = static_cast<char*>(p.y) + ((long long)(rt * BM + r) * p.ldy + n) * (OUT == OUT_F32 ? 4 : 2);
+        if (n + 4 <= p.N && p.tma_out) {
+          if (OUT == OUT_F32) *reinterpret_cast<float4*>(at) = v;
+          if (OUT == OUT_BF16) *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+          if (OUT == OUT_F16) *reinterpret_cast<uint2*>(at) = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+        } else {
+          if (n < p.N) store_one<OUT>(at, 0, v.x);
+          if (n + 1 < p.N) store_one<OUT>(at, 1, v.y);
+          if (n + 2 < p.N) store_one<OUT>(at, 2, v.z);
+          if (n + 3 < p.N) store_one<OUT>(at, 3, v.w);
+        }
+      }
+    }
+  }
+  if (csize > 1) cluster_sync_all();               // a peer may still read this CTA's memory or signal its barriers
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_512<CG>(tmem);
 }
 
+// One warp per row: the column groups' statistics merged.
 __global__ void __launch_bounds__(128)
     head_merge_kernel(const float* __restrict__ part, const float* __restrict__ token,
-                      const long long* __restrict__ ids, int tiles, int M, int N, float* logprob, float* entropy,
+                      const long long* __restrict__ ids, int groups, int M, int N, float* logprob, float* entropy,
                       float* lse) {
   const int m = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (m >= M) return;
   LogitStat st = logit_stat_empty();
-  for (int t = threadIdx.x & 31; t < tiles; t += 32) {
+  for (int t = threadIdx.x & 31; t < groups; t += 32) {
     const float* o = part + (long long)t * 3 * M + m;
     st = logit_stat_merge(st, LogitStat{o[0], o[M], o[2LL * M]});
   }
@@ -140,18 +541,166 @@ __global__ void __launch_bounds__(128)
   }
 }
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// ---- host -----------------------------------------------------------------------------------------
+
+struct Operands {
+  const void* x;
+  long long ldx;
+  const float* xs;
+  long long xs_row, xs_col;
+  const void* w;
+  long long ldw;
+  int packed;
+  const float* ws;
+  long long ws_row;
+  int M, N, K;
+};
+
+bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check_operands(const Operands& p) {
   if (p.M < 0) return -1;
   if (p.N < 1 || (p.packed && p.N % 16)) return -2;
   if (p.K < 16 || p.K % 16 || (p.packed && p.K % 128)) return -3;
   if (p.ldx < p.K || p.ldx % 16 || (!p.packed && (p.ldw < p.K || p.ldw % 16))) return -4;
-  if (!aligned16(p.x) || !aligned16(p.w)) return -10;
+  if (!aligned(p.x, 16) || !aligned(p.w, 16)) return -10;
   return 0;
 }
 
-int column_tiles(int N) { return (N + T - 1) / T; }
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// rows x K bytes, row-major: boxes of box_rows x 128 B landing as [box_rows][128 B], 128-byte swizzled.
+int rows_map(CUtensorMap* m, const void* base, int rows, int K, long long ld, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, es[2] = {1, 1};
+  const auto fn = encoder();
+  if (fn == nullptr) return -12;
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
+}
+
+// The strip pack [N/16][K/128][16 rows][128 B], already swizzled: (byte, row, strip, 128-K block).
+int strips_map(CUtensorMap* m, const void* base, int N, int K, int box_rows) {
+  const int KB = K / 128;
+  const cuuint64_t dims[4] = {128, 16, (cuuint64_t)(N / 16), (cuuint64_t)KB};
+  const cuuint64_t strides[3] = {128, (cuuint64_t)KB * 2048, 2048};
+  const cuuint32_t box[4] = {128, 16, (cuuint32_t)(box_rows / 16), 1}, es[4] = {1, 1, 1, 1};
+  const auto fn = encoder();
+  if (fn == nullptr) return -12;
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
+}
+
+// y [rows, cols] of 2 or 4-byte elements: boxes of 32 rows x 64 B, 64-byte swizzled.
+int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld * es : ((long long)cols * es + 15) / 16 * 16)};
+  const cuuint32_t box[2] = {(cuuint32_t)(64 / es), 32}, one[2] = {1, 1};
+  const auto fn = encoder();
+  if (fn == nullptr) return -12;
+  return fn(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box,
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
+}
+
+constexpr int MAX_DEVICES = 64;
+
+int num_sms() {
+  static int cached[MAX_DEVICES] = {};
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 148;
+  if (cached[dev] <= 0)
+    cached[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
+  return cached[dev];
+}
+
+template <int CG, int BN, int OUT>
+int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
+  constexpr int B_ROWS = BN / CG, STAGE = (BM + B_ROWS) * 128;
+  p.xs = o.xs, p.xs_row = o.xs_row, p.xs_col = o.xs_col, p.ws = o.ws, p.ws_row = o.ws_row;
+  p.M = o.M, p.N = o.N, p.K = o.K, p.packed = o.packed;
+  p.box_m = std::min(BM, (o.M + 7) / 8 * 8);
+  p.row_tiles = (o.M + BM * CG - 1) / (BM * CG);
+  p.col_tiles = (o.N + BN - 1) / BN;
+  if ((long long)p.row_tiles * p.col_tiles > (1 << 30)) return -8;
+  CUtensorMap xmap, wmap, ymap{};
+  int rc = rows_map(&xmap, o.x, o.M, o.K, o.ldx, p.box_m);
+  if (rc == 0) rc = o.packed ? strips_map(&wmap, o.w, o.N, o.K, B_ROWS) : rows_map(&wmap, o.w, o.N, o.K, o.ldw, B_ROWS);
+  if (rc == 0 && OUT != OUT_STATS && p.tma_out) rc = out_map(&ymap, p.y, o.M, o.N, p.ldy, OUT == OUT_F32 ? 4 : 2);
+  if (rc != 0) return rc;
+  const int tiles = p.row_tiles * p.col_tiles, KB = (o.K + 127) / 128;
+  const int cl = CG == 2 ? 2 : split;
+  const int clusters = cl == 1 || CG == 2 ? std::min(tiles, num_sms() / cl) : tiles;
+  const int per_cta = CG == 2 || split == 1 ? (tiles + clusters - 1) / clusters * KB : (KB + split - 1) / split;
+  p.nstage = std::min({MAX_STAGES, (SMEM_CAP - 1024 - ring_offset<OUT>()) / STAGE, std::max(2, per_cta)});
+  int smem = std::max(SMEM_MIN, 1024 + ring_offset<OUT>() + p.nstage * STAGE);
+  if (split > 1) smem = std::max(smem, 1024 + ring_offset<OUT>() + BM * (BN + 4) * 4);
+  auto kern = product_kernel<CG, BN, OUT>;
+  static bool ready[MAX_DEVICES] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= MAX_DEVICES || !ready[dev]) {
+    if (Tile<BN>::SPLIT_REGS) {                       // the split's sum must be what the launch brings
+      cudaFuncAttributes fa;
+      e = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(kern));
+      if (e != cudaSuccess) return (int)e;
+      if (fa.numRegs != Tile<BN>::LAUNCH_REGS) return -13;
+    }
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_CAP);
+    if (e != cudaSuccess) return (int)e;
+    if (dev < MAX_DEVICES) ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(clusters * cl);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cl;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, xmap, wmap, ymap, p);
+  return (int)(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+template <int OUT>
+int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
+  // Columns of a tile and CTAs that split its K: the fewest tile steps on the busiest SM, at the measured
+  // clocks of a 128-K block (430, 650, 1000 for 64, 128, 256 columns) and of a cluster's final sum.
+  const int KB = (o.K + 127) / 128, rows = (o.M + BM - 1) / BM, sms = num_sms();
+  int bn = 256, split = 1;
+  double best = 1e30;
+  for (int b = 64; b <= 256; b *= 2)
+    for (int s = 1; s <= (OUT == OUT_STATS || b == 256 ? 1 : 8) && s <= KB; s *= 2) {
+      if (OUT == OUT_STATS && b != 256) continue;
+      const long long ctas = (long long)rows * ((o.N + b - 1) / b) * s;
+      if (s > 1 && ctas > sms) continue;
+      const double waves = (double)((ctas + sms - 1) / sms);
+      const double t = waves * ((KB + s - 1) / s) * (b == 64 ? 430. : b == 128 ? 650. : 1000.) + (s > 1 ? 2000. : 0.);
+      if (t < best) best = t, bn = b, split = s;
+    }
+  if (bn == 256) return launch<1, 256, OUT>(o, p, 1, stream);
+  if (bn == 128) return launch<1, 128, OUT>(o, p, split, stream);
+  return launch<1, 64, OUT>(o, p, split, stream);
+}
+
+constexpr int GROUP = 256;                          // columns of one part of the head's statistics
+int column_groups(int N) { return (N + GROUP - 1) / GROUP; }
 
 }  // namespace
 
@@ -160,44 +709,44 @@ extern "C" {
 int b200_fp8_block_gemm(const void* qx, long long ldx, const float* xs, long long xs_row, long long xs_col,
                         const void* wq, long long ldw, int packed, const float* ws, long long ws_row, void* y,
                         long long ldy, int y_dtype, int M, int N, int K, cudaStream_t stream) {
-  const Operands p{static_cast<const uint8_t*>(qx), ldx, xs, xs_row, xs_col, static_cast<const uint8_t*>(wq), ldw,
-                   packed, ws, ws_row, M, N, K};
-  const int rc = check_operands(p);
+  const Operands o{qx, ldx, xs, xs_row, xs_col, wq, ldw, packed, ws, ws_row, M, N, K};
+  const int rc = check_operands(o);
   if (rc != 0) return rc;
   if (ldy < N) return -4;
   if (y_dtype < 0 || y_dtype > 2) return -5;
-  if (reinterpret_cast<uintptr_t>(y) & (y_dtype == 2 ? 3 : 1)) return -10;
+  const int es = y_dtype == 2 ? 4 : 2;
+  if (!aligned(y, es)) return -10;
   if (M == 0) return 0;
-  const dim3 grid(column_tiles(N), (M + T - 1) / T);
-  if (y_dtype == 0)
-    gemm_kernel<<<grid, 256, 0, stream>>>(p, static_cast<__nv_bfloat16*>(y), ldy);
-  else if (y_dtype == 1)
-    gemm_kernel<<<grid, 256, 0, stream>>>(p, static_cast<__half*>(y), ldy);
-  else
-    gemm_kernel<<<grid, 256, 0, stream>>>(p, static_cast<float*>(y), ldy);
-  return (int)cudaGetLastError();
+  Product p{};
+  p.y = y;
+  p.ldy = ldy;
+  p.tma_out = aligned(y, 16) && (M == 1 || ldy * es % 16 == 0);
+  return y_dtype == 0 ? launch_product<OUT_BF16>(o, p, stream)
+                      : y_dtype == 1 ? launch_product<OUT_F16>(o, p, stream) : launch_product<OUT_F32>(o, p, stream);
 }
 
 long long b200_fp8_head_logprobs_workspace_bytes(int M, int N) {
   if (M <= 0 || N <= 0) return 0;
-  return (3LL * column_tiles(N) + 1) * M * 4;
+  return (3LL * column_groups(N) + 1) * M * 4;
 }
 
 int b200_fp8_head_logprobs(const void* qx, long long ldx, const float* xs, long long xs_row, long long xs_col,
                            const void* wq, long long ldw, int packed, const float* ws, long long ws_row,
                            const long long* ids, int M, int N, int K, float* logprob, float* entropy, float* lse,
                            void* workspace, long long workspace_bytes, cudaStream_t stream) {
-  const Operands p{static_cast<const uint8_t*>(qx), ldx, xs, xs_row, xs_col, static_cast<const uint8_t*>(wq), ldw,
-                   packed, ws, ws_row, M, N, K};
-  const int rc = check_operands(p);
+  const Operands o{qx, ldx, xs, xs_row, xs_col, wq, ldw, packed, ws, ws_row, M, N, K};
+  int rc = check_operands(o);
   if (rc != 0) return rc;
   if (M == 0) return 0;
   if (workspace == nullptr || workspace_bytes < b200_fp8_head_logprobs_workspace_bytes(M, N)) return -9;
-  if (!aligned16(workspace)) return -10;
-  float* token = static_cast<float*>(workspace);
-  float* part = token + M;
-  head_kernel<<<dim3(column_tiles(N), (M + T - 1) / T), 256, 0, stream>>>(p, ids, part, token);
-  head_merge_kernel<<<(M + 3) / 4, 128, 0, stream>>>(part, token, ids, column_tiles(N), M, N, logprob, entropy, lse);
+  if (!aligned(workspace, 16)) return -10;
+  Product p{};
+  p.ids = ids;
+  p.token = static_cast<float*>(workspace);
+  p.part = p.token + M;
+  rc = launch_product<OUT_STATS>(o, p, stream);
+  if (rc != 0) return rc;
+  head_merge_kernel<<<(M + 3) / 4, 128, 0, stream>>>(p.part, p.token, ids, column_groups(N), M, N, logprob, entropy, lse);
   return (int)cudaGetLastError();
 }
 
