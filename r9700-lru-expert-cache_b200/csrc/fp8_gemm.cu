@@ -163,47 +163,47 @@ __device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* 
 }
 
 // A row's statistics over the W values of a group whose first column is n, and its token's logit if it is one.
+// Columns beyond N become -inf, which adds nothing.
 template <int W, bool SEG>
-__device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, const float2 (&acc)[W / 2]) {
-  auto at = [&](int c) { return c & 1 ? acc[c / 2].y : acc[c / 2].x; };
-  auto in = [&](int c) { return n + column<SEG>(c) < p.N; };
+__device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, float2 (&acc)[W / 2]) {
+  if (n + column<SEG>(W - 1) >= p.N) {
+#pragma unroll
+    for (int c = 0; c < W; c += 2) {
+      if (n + column<SEG>(c) >= p.N) acc[c / 2].x = -INFINITY;
+      if (n + column<SEG>(c + 1) >= p.N) acc[c / 2].y = -INFINITY;
+    }
+  }
   const long long id = p.ids[m] - n;
-  if (id >= 0 && id < column<SEG>(W - 1) + 1 && id < p.N - n) {
-    float v = NAN;
+  if (id >= 0 && id <= column<SEG>(W - 1) && id < p.N - n) {
+    uint32_t bits = 0;                               // (an indexed read would move the values to memory)
     bool mine = false;
 #pragma unroll
-    for (int c = 0; c < W; ++c)
-      if (column<SEG>(c) == (int)id) v = at(c), mine = true;
-    if (mine) p.token[m] = v;
+    for (int c = 0; c < W; ++c) {
+      const bool hit = column<SEG>(c) == (int)id;
+      bits |= __float_as_uint(c & 1 ? acc[c / 2].y : acc[c / 2].x) & (hit ? 0xffffffffu : 0u);
+      mine |= hit;
+    }
+    if (mine) p.token[m] = __uint_as_float(bits);
   }
   LogitStat st;
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  float odd[4] = {};                                 // NaN once a NaN or an infinity of either sign was seen
 #pragma unroll
-  for (int c = 0; c < W; ++c)
-    if (in(c)) {
-      mx[c & 3] = fmaxf(mx[c & 3], at(c));
-      odd[c & 3] = fmaf(at(c), 0.f, odd[c & 3]);
-    }
+  for (int c = 0; c < W / 2; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(acc[c].x, acc[c].y));
   st.m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  float s[4] = {}, w[4] = {};
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float s[2] = {}, w[2] = {};
 #pragma unroll
-  for (int c = 0; c < W; ++c) {
-    const float d = in(c) ? fmaxf(at(c) - st.m, -200.f) : -200.f;  // e^-200 = 0 in fp32, and 0 * -200 = 0
-    const float e = __expf(d);
-    s[c & 3] += e;
-    w[c & 3] = fmaf(e, d, w[c & 3]);
+  for (int c = 0; c < W / 2; ++c) {
+    const float dx = max_nan(acc[c].x - ref, -200.f), dy = max_nan(acc[c].y - ref, -200.f);  // e^-200 = 0 in fp32
+    const float ex = __expf(dx), ey = __expf(dy);
+    s[0] += ex;
+    s[1] += ey;
+    w[0] = fmaf(ex, dx, w[0]);
+    w[1] = fmaf(ey, dy, w[1]);
   }
-  st.s = (s[0] + s[1]) + (s[2] + s[3]);
-  st.w = (w[0] + w[1]) + (w[2] + w[3]);
-  if (st.m == -INFINITY) st.s = st.w = 0.f;
-  if (isnan((odd[0] + odd[1]) + (odd[2] + odd[3]))) {
-    // -inf beside finite values is as if it were absent; NaN and +inf make the row NaN
-    bool nan = st.m == INFINITY;
-#pragma unroll
-    for (int c = 0; c < W; ++c) nan |= in(c) && isnan(at(c));
-    if (nan) st = LogitStat{0.f, NAN, NAN};
-  }
+  st.s = s[0] + s[1];
+  st.w = w[0] + w[1];
+  if (isnan(st.s)) st = LogitStat{0.f, NAN, NAN};    // a NaN, or +inf (whose difference from itself is NaN)
   return st;
 }
 

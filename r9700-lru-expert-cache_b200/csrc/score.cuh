@@ -4,6 +4,13 @@
 
 namespace b200 {
 
+// The larger one; NaN if either is.
+B200_DEVINL float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Statistics of a row of logits relative to a reference m (its running maximum):
 // s = sum e^(x - m), w = sum e^(x - m) (x - m). m = -inf: nothing but -inf so far, s = w = 0.
 struct LogitStat {
