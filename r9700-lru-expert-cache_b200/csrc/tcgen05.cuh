@@ -141,6 +141,11 @@ B200_DEVINL uint32_t cluster_size() {
 B200_DEVINL void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+B200_DEVINL void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+B200_DEVINL void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+B200_DEVINL void st_cluster(uint32_t cluster_addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
 // The shared::cluster address of this CTA's shared address in CTA `rank` of the cluster.
 B200_DEVINL uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
   uint32_t r;
