@@ -29,6 +29,7 @@ constexpr int EPI_GROUPS = 2, EPI_WARPS = 4 * EPI_GROUPS;
 constexpr int THREADS = 32 * (4 + EPI_WARPS);
 constexpr int BM = 128;                    // token rows of a CTA's tile (TMEM lanes)
 constexpr int SMEM_CAP = 227 * 1024;
+constexpr int OUT_BUFS = 2, OUT_BUF = 4096; // a warp's output buffers: bf16 and f16 tiles fit whole
 constexpr int MAX_STAGES = 12;
 // Every CTA takes all of TMEM, so no two may share an SM (a second one's allocation would wait, and CTAs of
 // two clusters could wait for each other): each asks for more than half of the shared memory.
@@ -65,10 +66,10 @@ enum Out { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2, OUT_STATS = 3 };
 // next MMA takes longer than the other one's MMAs.
 template <int BN>
 struct Tile {
-    static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
+      static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
   static constexpr int UN = BN / UNITS;             // their columns
   static constexpr int W = BN / EPI_GROUPS;         // columns of one epilogue group
-  static constexpr int CHUNK = W < 32 ? W : 32;     // columns of one TMEM load
+  static constexpr int CHUNK = 16;                  // columns of one TMEM load
   static constexpr int NBUF = 512 / UN > 8 ? 8 : 512 / UN;
   static constexpr int RELEASERS = UNITS == 2 ? EPI_WARPS / 2 : EPI_WARPS;   // warps of a CTA that read one
   static constexpr int BLOCKS = BN > 128 ? BN / 128 : 1;   // weight scales of a tile's 128-K block
@@ -108,7 +109,15 @@ __device__ __forceinline__ void store_one(void* row, int col, float v) {
   if (OUT == OUT_F32) static_cast<float*>(row)[col] = v;
 }
 
-// Writes a warp's 32 rows x W columns of y at (m0, n0), 64 bytes a row at a time through one of two 2 KB
+// Output goes through shared memory in boxes of 32 rows, 128 or 64 bytes wide, in the tensor map's swizzled order:
+// 16-byte piece q of row r at piece q ^ (r mod 8) of 128, q ^ (r / 2 mod 4) of 64 bytes. No bank conflicts either way.
+__host__ __device__ constexpr int out_row_bytes(int bytes) { return bytes >= 128 ? 128 : 64; }
+template <int ROW>
+__device__ __forceinline__ int swizzled(int r, int q) {
+  return r * ROW + ((ROW == 128 ? q ^ (r & 7) : q ^ ((r >> 1) & 3)) << 4);
+}
+
+// Writes a warp's 32 rows x W columns of y at (m0, n0), up to 128 bytes a row at a time through one of two 4 KB
 // buffers: a tensor-map store that runs on while the warp goes back to its next tile (rows beyond M and columns
 // beyond N are clipped by the copy), or, where y's base or rows are not 16-byte aligned, plain coalesced stores.
 // Straight from registers, 32 rows an instruction, the same tile took 6400 clocks of the 10240 that its MMAs
@@ -116,15 +125,16 @@ __device__ __forceinline__ void store_one(void* row, int col, float v) {
 template <int OUT, int W, bool SEG>
 __device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* ymap, char* bufs, int& turn, int m0,
                                            int n0, int lane, const float2 (&acc)[W / 2]) {
-  constexpr int ES = OUT == OUT_F32 ? 4 : 2, CC = 64 / ES;
+  constexpr int ES = OUT == OUT_F32 ? 4 : 2;
+  constexpr int ROW = out_row_bytes(W * ES), CC = ROW / ES, Q = ROW / 16;   // bytes, columns and 16-byte pieces of a row
 #pragma unroll
   for (int c = 0; c < W; c += CC, ++turn) {
-    char* buf = bufs + (turn & 1) * 2048;
+    char* buf = bufs + (turn & (OUT_BUFS - 1)) * OUT_BUF;
     const int n = n0 + column<SEG>(c);
-    if (lane == 0) bulk_wait_read<1>();              // this buffer's last store has been read
+    if (lane == 0) bulk_wait_read<OUT_BUFS - 1>();   // this buffer's last store has been read
     __syncwarp();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < Q; ++q) {
       uint32_t v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -132,8 +142,7 @@ __device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* 
         if (OUT == OUT_BF16) v[i] = pack_bf16(acc[c / 2 + 4 * q + i].x, acc[c / 2 + 4 * q + i].y);
         if (OUT == OUT_F16) v[i] = pack_f16(acc[c / 2 + 4 * q + i].x, acc[c / 2 + 4 * q + i].y);
       }
-      // 64-byte swizzle: 16-byte piece q of row r at piece q ^ ((r / 2) mod 4)
-      *reinterpret_cast<uint4*>(buf + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+      *reinterpret_cast<uint4*>(buf + swizzled<ROW>(lane, q)) = make_uint4(v[0], v[1], v[2], v[3]);
     }
     if (p.tma_out) {
       fence_proxy_async_smem();
@@ -149,7 +158,7 @@ __device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* 
       for (int i = lane; i < 32 * CC; i += 32) {
         const int r = i / CC, col = i % CC;
         if (m0 + r < p.M && n + col < p.N) {
-          const char* from = buf + r * 64 + (((col * ES >> 4) ^ ((r >> 1) & 3)) << 4) + (col * ES & 15);
+          const char* from = buf + swizzled<ROW>(r, col * ES >> 4) + (col * ES & 15);
           char* to = y + ((long long)(m0 + r) * p.ldy + n + col) * ES;
           if (ES == 4)
             *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from);
@@ -211,7 +220,7 @@ __device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, f
 __host__ __device__ constexpr int out_offset() { return (1024 + 2 * FGROUP * F_LD * 4 + 1023) / 1024 * 1024; }
 template <int OUT>
 __host__ __device__ constexpr int ring_offset() {
-  return out_offset() + (OUT == OUT_STATS ? 2 * 3 * EPI_GROUPS * BM * 4 : EPI_WARPS * 4096);
+  return out_offset() + (OUT == OUT_STATS ? 2 * 3 * EPI_GROUPS * BM * 4 : EPI_WARPS * OUT_BUFS * OUT_BUF);
 }
 
 // One CTA (CG = 1; gridDim / cluster size clusters, whose CTAs split K) or one CTA pair (CG = 2).
@@ -395,6 +404,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int row_in_tile = 32 * quarter + lane;
     const float* my_factors = factors + (BN == 256 && !SEG ? group : 0) * BM + row_in_tile;
     const int col = SEG ? 64 * group : W * group;    // first column of the group in its tile
+    const uint32_t release = map_to_rank(smem_u32(acc_empty), CG == 2 ? 0 : cluster_rank());   // where the MMAs are issued
     int buf = UNITS == 2 ? group : 0, use = 0, turn = 0, fg = 0;
     bool ok = true;
     for (int t = first; t < tiles; t += step) {
@@ -412,26 +422,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float scale0 = now[0], scale1 = SEG ? now[BM] : scale0;
         const uint32_t src = lanes + buf * UN;
         constexpr int C = Tile<BN>::CHUNK;
-        uint32_t v[2][C];
-        tmem_ld<C>(src, v[0]);
 #pragma unroll
         for (int c = 0; c < W; c += C) {
-          uint32_t(&x)[C] = v[c / C & 1];
-          tmem_wait_ld<C>(x);
-          if (c + C < W) {
-            tmem_ld<C>(src + c + C, v[(c / C & 1) ^ 1]);
-          } else {
+          uint32_t v[C];
+          tmem_ld<C>(src + c, v);
+          tmem_wait_ld<C>(v);
+          if (c + C == W) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if (CG == 1 || rank == 0)
-                mbar_arrive(&acc_empty[buf]);
-              else
-                mbar_arrive_remote(map_to_rank(smem_u32(&acc_empty[buf]), 0));
-            }
+            if (lane == 0) mbar_arrive_remote(release + buf * 8);
           }
 #pragma unroll
-          for (int i = 0; i < C / 2; ++i) fma2_scaled(acc[c / 2 + i], x[2 * i], x[2 * i + 1], c < 64 ? scale0 : scale1);
+          for (int i = 0; i < C / 2; ++i) fma2_scaled(acc[c / 2 + i], v[2 * i], v[2 * i + 1], c < 64 ? scale0 : scale1);
         }
         if (fi == FGROUP - 1 || kb + 1 == kb1) {
           __syncwarp();
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         ++turn;
       } else if (ok && split == 1 && n < p.N && m - lane < p.M) {
-        store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (warp - 4) * 4096, turn, m - lane, n, lane, acc);
+        store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (warp - 4) * OUT_BUFS * OUT_BUF, turn, m - lane, n, lane, acc);
       }
     }
     if (OUT != OUT_STATS && lane == 0) bulk_wait_all();
@@ -603,15 +605,15 @@ int strips_map(CUtensorMap* m, const void* base, int N, int K, int box_rows) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
 }
 
-// y [rows, cols] of 2 or 4-byte elements: boxes of 32 rows x 64 B, 64-byte swizzled.
-int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es) {
+// y [rows, cols] of 2 or 4-byte elements: boxes of 32 rows x row_bytes, swizzled.
+int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es, int row_bytes) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld * es : ((long long)cols * es + 15) / 16 * 16)};
-  const cuuint32_t box[2] = {(cuuint32_t)(64 / es), 32}, one[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)(row_bytes / es), 32}, one[2] = {1, 1};
   const auto fn = encoder();
   if (fn == nullptr) return -12;
   return fn(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box,
-            one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
 }
 
@@ -638,7 +640,8 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   CUtensorMap xmap, wmap, ymap{};
   int rc = rows_map(&xmap, o.x, o.M, o.K, o.ldx, p.box_m);
   if (rc == 0) rc = o.packed ? strips_map(&wmap, o.w, o.N, o.K, B_ROWS) : rows_map(&wmap, o.w, o.N, o.K, o.ldw, B_ROWS);
-  if (rc == 0 && OUT != OUT_STATS && p.tma_out) rc = out_map(&ymap, p.y, o.M, o.N, p.ldy, OUT == OUT_F32 ? 4 : 2);
+  if (rc == 0 && OUT != OUT_STATS && p.tma_out) rc = out_map(&ymap, p.y, o.M, o.N, p.ldy, OUT == OUT_F32 ? 4 : 2,
+                                                             out_row_bytes(Tile<BN>::W * (OUT == OUT_F32 ? 4 : 2)));
   if (rc != 0) return rc;
   const int tiles = p.row_tiles * p.col_tiles, KB = (o.K + 127) / 128;
   const int cl = CG == 2 ? 2 : split;
@@ -694,7 +697,7 @@ int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
       const double t = waves * ((KB + s - 1) / s) * (b == 64 ? 430. : b == 128 ? 650. : 1000.) + (s > 1 ? 2000. : 0.);
       if (t < best) best = t, bn = b, split = s;
     }
-  if (bn == 256) return launch<1, 256, OUT>(o, p, 1, stream);
+  if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, 1, stream) : launch<1, 256, OUT>(o, p, 1, stream);
   if (bn == 128) return launch<1, 128, OUT>(o, p, split, stream);
   return launch<1, 64, OUT>(o, p, split, stream);
 }
