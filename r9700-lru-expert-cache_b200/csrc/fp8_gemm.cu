@@ -8,7 +8,7 @@
 // thread that holds a lane's columns needs ONE factor per block: the promotion of D_b into the running sum is
 // a tcgen05.ld and one fused multiply-add per value, in registers, while the MMAs fill the other accumulators.
 //   warp 0     one lane copies the tiles (tensor maps: zeros beyond M, N and K) into a ring of stages;
-//   warp 1     one lane issues the MMAs, four of K = 32 a stage, a fresh accumulator for every 128-K block;
+//   warps 1, 3 one lane each issues MMAs, four of K = 32 a 128-K block, into a fresh accumulator;
 //   warp 2     puts the factors xs ws of four 128-K blocks at a time into shared memory;
 //   warps 4-11 two groups of four, each with half of the columns: promote, then write the tile.
 // CTAs (or pairs) walk the tiles, rows first within groups of row tiles, so that tiles in flight share weights.
@@ -52,9 +52,9 @@ struct Product {
   void* y;
   long long ldy;
   int tma_out;                             // y's base and rows are 16-byte aligned
-  // head: part [column group][3][M], token [M]
+  // head: of every row and column tile {m, s, w, 0}; of every row its token's logit
   const long long* ids;
-  float* part;
+  float4* part;
   float* token;
 };
 
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* f_full = acc_empty + 8;
   uint64_t* f_empty = f_full + 2;
   uint64_t* done = f_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   float* factors = reinterpret_cast<float*>(sm + 1024);
   float* stat_s = reinterpret_cast<float*>(sm + out_offset());      // head: [2][3][EPI_GROUPS][BM]
   char* ring = sm + ring_offset<OUT>();
@@ -255,10 +255,44 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int first = blockIdx.x / csize, step = gridDim.x / csize;
   const int nstage = p.nstage;
 
+  // The copies' place in the CTA's blocks: thread 0 alone moves it.
+  const uint32_t rank = CG == 2 ? crank : 0;
+  struct {
+    int t, kb, m, n, s, round;
+    long long count;
+  } at;
+  auto to_tile = [&](int t) {
+    int rt, ct;
+    tile_at(p, t, rt, ct);
+    at.t = t;
+    at.kb = kb0;
+    at.m = (rt * CG + (int)rank) * BM;
+    at.n = ct * BN + (int)rank * B_ROWS;
+  };
+  auto copy_next = [&]() {                           // the next block into stage at.s, which is free
+    uint32_t bar = smem_u32(&full[at.s]);
+    if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[at.s], (uint32_t)(p.box_m + B_ROWS) * 128 * CG);
+    if (CG == 2) bar = map_to_rank(bar, 0);
+    const uint32_t dst = smem_u32(ring + at.s * STAGE);
+    tma_load_2d<CG>(dst, &xmap, at.kb * 128, at.m, bar);
+    if (p.packed)
+      tma_load_4d<CG>(dst + BM * 128, &wmap, 0, 0, at.n / 16, at.kb, bar);
+    else
+      tma_load_2d<CG>(dst + BM * 128, &wmap, at.kb * 128, at.n, bar);
+    ++at.count;
+    if (++at.s == nstage) at.s = 0, ++at.round;
+    if (++at.kb == kb1) {
+      at.t += step;
+      if (at.t < tiles) to_tile(at.t);
+    }
+  };
+  if (CG == 1 && csize > 1) cluster_arrive();        // (waited for before the first store to another CTA)
   if (threadIdx.x == 0) {
+    prefetch_map(&xmap);
+    prefetch_map(&wmap);
     for (int i = 0; i < nstage; ++i) {
       mbar_init(&full[i], 1);
-      mbar_init(&empty[i], UNITS);
+      mbar_init(&empty[i], UNITS);                   // a commit of each issuer that reads the stage
     }
     for (int i = 0; i < NBUF; ++i) {
       mbar_init(&acc_full[i], 1);
@@ -268,98 +302,89 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&f_full[i], 1);
       mbar_init(&f_empty[i], EPI_WARPS);
     }
-    mbar_init(done, UNITS);
+    mbar_init(&done[0], 1);
+    mbar_init(&done[1], 1);
     fence_mbar_init();
+    at.s = at.round = 0;
+    at.count = 0;
+    to_tile(first);
+    // The first ring of copies goes out before the rest of the CTA is set up (a pair's needs the other CTA's barriers).
+    if (CG == 1)
+      while (at.t < tiles && at.round == 0) copy_next();
   }
   if (warp == 1) tmem_alloc_512<CG>(tmem_slot);
   tc_fence_before();
   __syncthreads();
-  if (csize > 1) cluster_sync_all();
+  if (CG == 2) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (OUT == OUT_STATS) griddep_launch_dependents();  // the merge may take its place as SMs free up
 
   float2 acc[W / 2];
   if (Tile<BN>::SPLIT_REGS && warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Tile<BN>::OTHER_REGS));
   if (warp == 0) {
     if (lane == 0) {
       // ---------------- copies ----------------
-      const uint32_t rank = CG == 2 ? crank : 0;
-      const uint32_t bytes = (p.box_m + B_ROWS) * 128 * CG;
-      int it = 0, s = 0, round = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        int rt, ct;
-        tile_at(p, t, rt, ct);
-        const int m = (rt * CG + (int)rank) * BM, n = ct * BN + (int)rank * B_ROWS;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          if (round > 0 && !mbar_wait_limited(&empty[s], (round - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          uint32_t bar = smem_u32(&full[s]);
-          if (CG == 1 || rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-          if (CG == 2) bar = map_to_rank(bar, 0);
-          const uint32_t dst = smem_u32(ring + s * STAGE);
-          tma_load_2d<CG>(dst, &xmap, kb * 128, m, bar);
-          if (p.packed)
-            tma_load_4d<CG>(dst + BM * 128, &wmap, 0, 0, n / 16, kb, bar);
-          else
-            tma_load_2d<CG>(dst + BM * 128, &wmap, kb * 128, n, bar);
-          if (++s == nstage) s = 0, ++round;
-        }
+      while (at.t < tiles && ok) {
+        ok = at.round == 0 || mbar_wait_limited(&empty[at.s], (at.round - 1) & 1);
+        if (ok) copy_next();
       }
       // Leave only when this CTA's copies have landed and been read: the MMAs' commit of each stage's last use.
-      const int last = min(it, nstage);
-      for (int i = 0; i < last && ok; ++i) {
-        const int q = it - last + i;
-        ok = mbar_wait_limited(&empty[q % nstage], (q / nstage) & 1);
-      }
+      const long long oldest = at.count > nstage ? at.count - nstage : 0;
+      for (long long q = oldest; q < at.count && ok; ++q)
+        ok = mbar_wait_limited(&empty[q % nstage], (uint32_t)(q / nstage) & 1);
       if (!ok) {
         atomicExch(&g_score_err, 1);
         if (CG == 1 || rank == 0)
-          for (int i = 0; i < last; ++i) mbar_wait_limited(&full[(it - last + i) % nstage], ((it - last + i) / nstage) & 1);
+          for (long long q = oldest; q < at.count; ++q) mbar_wait_limited(&full[q % nstage], (uint32_t)(q / nstage) & 1);
         else                                           // the pair's barriers are the other CTA's: time for any copy to land
           for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000ull;) __nanosleep(1000);
       }
     }
     __syncwarp();
-  } else if (warp == 1 || (UNITS == 2 && warp == 3)) {
+  } else if (warp == 1 || warp == 3) {
     if (CG == 1 || crank == 0) {
-      // ---------------- MMAs: warp 1 the first accumulator of a block, warp 3 the second one ----------------
-      // The whole warp walks the loop and one elected lane issues.
+      // ---------------- MMAs ----------------
+      // Two issuers, since a block's wait, four MMAs and two commits take a warp about 500 clocks: of a block's two
+      // accumulators one each (BN = 256), else every other block. The whole warp walks the loop and one elected
+      // lane issues.
       const uint32_t idesc = (1u << 4)                             // D: f32
                              | ((uint32_t)(UN >> 3) << 17)         // N
                              | ((uint32_t)(BM * CG >> 4) << 24);   // M; A, B: e4m3, K-major
       const int u = warp >> 1;
-      int s = 0, round = 0, buf = u, use = 0;
+      constexpr int STEP = UNITS == 2 ? 1 : 2;                     // blocks
+      const uint32_t b_offset = UNITS == 2 ? u * (UN / CG * 128) : 0;
+      const long long blocks = first < tiles ? (long long)((tiles - first + step - 1) / step) * (kb1 - kb0) : 0;
+      int s = UNITS == 2 ? 0 : u, round = 0, buf = u, use = 0;
+      if (s >= nstage) s -= nstage, ++round;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += step) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          ok = warp_wait(&full[s], round & 1, &acc_empty[buf], (use - 1) & 1, use > 0);
-          if (!ok) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t st = smem_u32(ring + s * STAGE);
-            const uint64_t a = sw128_desc(st), b = sw128_desc(st + BM * 128 + u * (UN / CG * 128));
-            const uint32_t d = tmem + buf * UN;
+      for (long long i = UNITS == 2 ? 0 : u; i < blocks; i += STEP) {
+        ok = warp_wait(&full[s], round & 1, &acc_empty[buf], (use - 1) & 1, use > 0);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t st = smem_u32(ring + s * STAGE);
+          const uint64_t a = sw128_desc(st), b = sw128_desc(st + BM * 128 + b_offset);
+          const uint32_t d = tmem + buf * UN;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc_mma_f8<CG>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : 0u);
-            tc_commit<CG>(&acc_full[buf]);
-            tc_commit<CG>(&empty[s]);
-          }
-          __syncwarp();
-          if (++s == nstage) s = 0, ++round;
-          buf += UNITS;
-          if (buf >= NBUF) buf -= NBUF, ++use;
+          for (int k = 0; k < 4; ++k) tc_mma_f8<CG>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : 0u);
+          tc_commit<CG>(&acc_full[buf]);
+          tc_commit<CG>(&empty[s]);
         }
+        __syncwarp();
+        s += STEP;
+        if (s >= nstage) s -= nstage, ++round;
+        buf += 2;
+        if (buf >= NBUF) buf -= NBUF, ++use;
       }
       if (!ok) {                                       // what was issued still writes TMEM
         if (elect_one()) {
           atomicExch(&g_score_err, 1);
-          tc_commit<CG>(done);
+          tc_commit<CG>(&done[u]);
         }
         __syncwarp();
-        mbar_wait_limited(done, 0);
+        mbar_wait_limited(&done[u], 0);
       }
     }
     __syncwarp();
@@ -367,7 +392,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------- factors ----------------
     // Lane = (row mod 8, block of the group): row-major scales are read 16 B a row, four blocks in one pass.
     const int r8 = lane >> 2, i = lane & 3;
-    const uint32_t rank = CG == 2 ? crank : 0;
     int fg = 0;
     bool ok = true;
     for (int t = first; t < tiles && ok; t += step) {
@@ -399,7 +423,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ---------------- promotion and output ----------------
     if constexpr (Tile<BN>::SPLIT_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Tile<BN>::EPI_REGS));
     const int quarter = warp & 3, group = (warp >> 2) - 1;
-    const uint32_t rank = CG == 2 ? crank : 0;
     const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + (UNITS == 1 ? group * W : 0);
     const int row_in_tile = 32 * quarter + lane;
     const float* my_factors = factors + (BN == 256 && !SEG ? group : 0) * BM + row_in_tile;
@@ -456,10 +479,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int g = 1; g < EPI_GROUPS; ++g)
             st = logit_stat_merge(st, LogitStat{own[g * BM], own[(EPI_GROUPS + g) * BM], own[(2 * EPI_GROUPS + g) * BM]});
-          float* o = p.part + (long long)ct * 3 * p.M + m;
-          o[0] = st.m;
-          o[p.M] = st.s;
-          o[2LL * p.M] = st.w;
+          p.part[(long long)m * p.col_tiles + ct] = make_float4(st.m, st.s, st.w, 0.f);
         }
         ++turn;
       } else if (ok && split == 1 && n < p.N && m - lane < p.M) {
@@ -472,70 +492,80 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   if constexpr (CAN_SPLIT) {
-    // ---------------- K split over the cluster's CTAs: one tile, whose ring is idle now ----------------
+    // ---------------- K split over the cluster's CTAs: one tile ----------------
+    // Each CTA owns BN / split of the columns: the others push their sums of those into its output buffers, which
+    // nothing else uses here, and it adds them in rank order.
     if (split > 1) {
-      constexpr int LD = BN + 4;
-      float* sums = reinterpret_cast<float*>(ring);
+      const int share = BN / split;
+      float* sums = reinterpret_cast<float*>(sm + out_offset());       // [split][BM][share]
+      static_assert(BM * BN * 4 <= EPI_WARPS * OUT_BUFS * OUT_BUF, "the output buffers hold a tile");
       int rt, ct;
       tile_at(p, first, rt, ct);
       const int rows = min(BM, p.M - rt * BM);
+      cluster_wait();                                // every CTA has started
       if (warp >= 4) {
         const int group = (warp >> 2) - 1, r = 32 * (warp & 3) + lane;
         if (r < rows) {
 #pragma unroll
-          for (int c = 0; c < W; c += 4)
-            *reinterpret_cast<float4*>(sums + r * LD + group * W + c) =
-                make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y);
+          for (int c = 0; c < W; c += 4) {
+            const int col = group * W + c, owner = col / share;
+            st_cluster_f4(map_to_rank(smem_u32(sums + (part * BM + r) * share + col - owner * share), owner),
+                          make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y));
+          }
         }
       }
       cluster_sync_all();
-      // each CTA adds, in rank order, its share of the columns
-      const int share = BN / split, quads = share / 4;
-      const uint32_t mine = smem_u32(sums);
+      const int quads = share / 4;
       for (int e = threadIdx.x; e < rows * quads; e += THREADS) {
-        const int r = e / quads, c = part * share + (e - r * quads) * 4;
+        const int r = e / quads, c = (e - r * quads) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t q = 0; q < split; ++q) {
-          const float4 u = ld_cluster_f4(map_to_rank(mine + (r * LD + c) * 4, q));
+          const float4 u = *reinterpret_cast<const float4*>(sums + (q * BM + r) * share + c);
           v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
         }
-        const int n = ct * BN + c;
-        char* at = static_cast<char*>(p.y) + ((long long)(rt * BM + r) * p.ldy + n) * (OUT == OUT_F32 ? 4 : 2);
+        const int n = ct * BN + part * share + c;
+        char* to = static_cast<char*>(p.y) + ((long long)(rt * BM + r) * p.ldy + n) * (OUT == OUT_F32 ? 4 : 2);
         if (n + 4 <= p.N && p.tma_out) {
-          if (OUT == OUT_F32) *reinterpret_cast<float4*>(at) = v;
-          if (OUT == OUT_BF16) *reinterpret_cast<uint2*>(at) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
-          if (OUT == OUT_F16) *reinterpret_cast<uint2*>(at) = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
+          if (OUT == OUT_F32) *reinterpret_cast<float4*>(to) = v;
+          if (OUT == OUT_BF16) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+          if (OUT == OUT_F16) *reinterpret_cast<uint2*>(to) = make_uint2(pack_f16(v.x, v.y), pack_f16(v.z, v.w));
         } else {
-          if (n < p.N) store_one<OUT>(at, 0, v.x);
-          if (n + 1 < p.N) store_one<OUT>(at, 1, v.y);
-          if (n + 2 < p.N) store_one<OUT>(at, 2, v.z);
-          if (n + 3 < p.N) store_one<OUT>(at, 3, v.w);
+          if (n < p.N) store_one<OUT>(to, 0, v.x);
+          if (n + 1 < p.N) store_one<OUT>(to, 1, v.y);
+          if (n + 2 < p.N) store_one<OUT>(to, 2, v.z);
+          if (n + 3 < p.N) store_one<OUT>(to, 3, v.w);
         }
       }
     }
   }
-  if (csize > 1) cluster_sync_all();               // a peer may still read this CTA's memory or signal its barriers
+  if (CG == 2) cluster_sync_all();                 // the other CTA may still signal this one's barriers
   tc_fence_after();
   if (warp == 1) tmem_dealloc_512<CG>(tmem);
 }
 
-// One warp per row: the column groups' statistics merged.
-__global__ void __launch_bounds__(128)
-    head_merge_kernel(const float* __restrict__ part, const float* __restrict__ token,
-                      const long long* __restrict__ ids, int groups, int M, int N, float* logprob, float* entropy,
-                      float* lse) {
-  const int m = blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (m >= M) return;
+// One CTA per row: the column tiles' statistics merged. Launched as the product's programmatic dependent.
+constexpr int MERGE_THREADS = 128;
+__global__ void __launch_bounds__(MERGE_THREADS)
+    head_merge_kernel(const float4* __restrict__ part, const float* __restrict__ token,
+                      const long long* __restrict__ ids, int tiles, int N, float* logprob, float* entropy, float* lse) {
+  __shared__ LogitStat sh[MERGE_THREADS / 32];
+  const int m = blockIdx.x;
+  const long long id = ids[m];
+  griddep_wait();
   LogitStat st = logit_stat_empty();
-  for (int t = threadIdx.x & 31; t < groups; t += 32) {
-    const float* o = part + (long long)t * 3 * M + m;
-    st = logit_stat_merge(st, LogitStat{o[0], o[M], o[2LL * M]});
+  for (int t = threadIdx.x; t < tiles; t += MERGE_THREADS) {
+    const float4 o = part[(long long)m * tiles + t];
+    st = logit_stat_merge(st, LogitStat{o.x, o.y, o.z});
   }
+#pragma unroll
   for (int o = 16; o; o >>= 1)
     st = logit_stat_merge(st, LogitStat{__shfl_xor_sync(~0u, st.m, o), __shfl_xor_sync(~0u, st.s, o),
                                         __shfl_xor_sync(~0u, st.w, o)});
-  if ((threadIdx.x & 31) == 0) {
-    const bool valid = ids[m] >= 0 && ids[m] < N;
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < MERGE_THREADS / 32; ++i) st = logit_stat_merge(st, sh[i]);
+    const bool valid = id >= 0 && id < N;
     const RowResult r = logit_stat_finish(st, valid ? token[m] : 0.f, valid);
     logprob[m] = r.logprob;
     entropy[m] = r.entropy;
@@ -649,7 +679,6 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   const int per_cta = CG == 2 || split == 1 ? (tiles + clusters - 1) / clusters * KB : (KB + split - 1) / split;
   p.nstage = std::min({MAX_STAGES, (SMEM_CAP - 1024 - ring_offset<OUT>()) / STAGE, std::max(2, per_cta)});
   int smem = std::max(SMEM_MIN, 1024 + ring_offset<OUT>() + p.nstage * STAGE);
-  if (split > 1) smem = std::max(smem, 1024 + ring_offset<OUT>() + BM * (BN + 4) * 4);
   auto kern = product_kernel<CG, BN, OUT>;
   static bool ready[MAX_DEVICES] = {};
   int dev = 0;
@@ -681,29 +710,29 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
+constexpr int HEAD_BN = 256;                        // columns of a head tile, which leave one set of statistics a row
+int head_tiles(int N) { return (N + HEAD_BN - 1) / HEAD_BN; }
+
 template <int OUT>
 int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
   // Columns of a tile and CTAs that split its K: the fewest tile steps on the busiest SM, at the measured
-  // clocks of a 128-K block (430, 650, 1000 for 64, 128, 256 columns) and of a cluster's final sum.
+  // clocks of a 128-K block (320, 540, 900 for 64, 128, 256 columns) and of a cluster's final sum.
   const int KB = (o.K + 127) / 128, rows = (o.M + BM - 1) / BM, sms = num_sms();
   int bn = 256, split = 1;
   double best = 1e30;
   for (int b = 64; b <= 256; b *= 2)
     for (int s = 1; s <= (OUT == OUT_STATS || b == 256 ? 1 : 8) && s <= KB; s *= 2) {
-      if (OUT == OUT_STATS && b != 256) continue;
+      if (OUT == OUT_STATS && b != HEAD_BN) continue;
       const long long ctas = (long long)rows * ((o.N + b - 1) / b) * s;
       if (s > 1 && ctas > sms) continue;
       const double waves = (double)((ctas + sms - 1) / sms);
-      const double t = waves * ((KB + s - 1) / s) * (b == 64 ? 430. : b == 128 ? 650. : 1000.) + (s > 1 ? 2000. : 0.);
+      const double t = waves * ((KB + s - 1) / s) * (b == 64 ? 320. : b == 128 ? 540. : 900.) + (s > 1 ? 2000. : 0.);
       if (t < best) best = t, bn = b, split = s;
     }
   if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, 1, stream) : launch<1, 256, OUT>(o, p, 1, stream);
   if (bn == 128) return launch<1, 128, OUT>(o, p, split, stream);
   return launch<1, 64, OUT>(o, p, split, stream);
 }
-
-constexpr int GROUP = 256;                          // columns of one part of the head's statistics
-int column_groups(int N) { return (N + GROUP - 1) / GROUP; }
 
 }  // namespace
 
@@ -730,7 +759,7 @@ int b200_fp8_block_gemm(const void* qx, long long ldx, const float* xs, long lon
 
 long long b200_fp8_head_logprobs_workspace_bytes(int M, int N) {
   if (M <= 0 || N <= 0) return 0;
-  return (3LL * column_groups(N) + 1) * M * 4;
+  return (16LL * head_tiles(N) + 4) * M;
 }
 
 int b200_fp8_head_logprobs(const void* qx, long long ldx, const float* xs, long long xs_row, long long xs_col,
@@ -745,12 +774,22 @@ int b200_fp8_head_logprobs(const void* qx, long long ldx, const float* xs, long 
   if (!aligned(workspace, 16)) return -10;
   Product p{};
   p.ids = ids;
-  p.token = static_cast<float*>(workspace);
-  p.part = p.token + M;
+  p.part = static_cast<float4*>(workspace);
+  p.token = reinterpret_cast<float*>(p.part + (long long)M * head_tiles(N));
   rc = launch_product<OUT_STATS>(o, p, stream);
   if (rc != 0) return rc;
-  head_merge_kernel<<<(M + 3) / 4, 128, 0, stream>>>(p.part, p.token, ids, column_groups(N), M, N, logprob, entropy, lse);
-  return (int)cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(M);
+  cfg.blockDim = dim3(MERGE_THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, head_merge_kernel, (const float4*)p.part, (const float*)p.token, ids,
+                                           head_tiles(N), N, logprob, entropy, lse);
+  return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
 int b200_score_error(int reset) {

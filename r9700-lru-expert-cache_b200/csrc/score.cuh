@@ -4,6 +4,11 @@
 
 namespace b200 {
 
+// Programmatic dependent launch: the dependent grid may be placed while its primary still runs; griddep_wait()
+// returns once the primary is complete and its writes are visible.
+B200_DEVINL void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+B200_DEVINL void griddep_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // The larger one; NaN if either is.
 B200_DEVINL float max_nan(float a, float b) {
   float r;

@@ -157,13 +157,9 @@ B200_DEVINL uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
 B200_DEVINL void mbar_arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
-B200_DEVINL float4 ld_cluster_f4(uint32_t cluster_addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(cluster_addr)
+B200_DEVINL void st_cluster_f4(uint32_t cluster_addr, float4 v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(cluster_addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w)
                : "memory");
-  return v;
 }
 
 // ---- bounded waits -----------------------------------------------------------------------------
@@ -199,6 +195,10 @@ B200_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity) {
 }
 
 // ---- tensor-map copies -------------------------------------------------------------------------
+
+B200_DEVINL void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 
 // One box global -> this CTA's shared memory, its bytes counted on the barrier at `bar` (a shared::cluster
 // address; for CG = 2 it may be the peer's).
