@@ -134,6 +134,17 @@ def stream_ptr(stream=None) -> c_vp:
     return c_vp(s.cuda_stream)
 
 
+def launch(fn, device, *args) -> int:
+    """fn(*args, stream) on the current stream of `device`, with `device` current. (The raw stream
+    handle: building a torch.cuda.Stream for it costs as much as the launch.)"""
+    import torch
+    index = device.index
+    if index == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed rc={rc}")

@@ -21,34 +21,42 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 def _operands(what: str, qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: torch.Tensor,
               packed: bool) -> tuple:
     """Checks the four operands and returns the C entries' leading arguments with M, N and K."""
-    _lib.require_cuda(what, qx, wq, xs, ws)
-    if qx.ndim != 2 or wq.ndim != 2 or qx.dtype != FP8 or wq.dtype != FP8:
+    dev = qx.device
+    if not qx.is_cuda or wq.device != dev or xs.device != dev or ws.device != dev:
+        _lib.require_cuda(what, qx, wq, xs, ws)
+        raise ValueError(f"{what}: operands are on different devices")
+    if qx.dtype is not FP8 or wq.dtype is not FP8 or qx.ndim != 2 or wq.ndim != 2:
         raise ValueError(f"{what}: qx and wq must be 2-D e4m3 tensors")
-    (M, K), N = qx.shape, wq.shape[0]
-    if wq.shape[1] != K:
+    M, K = qx.shape
+    N, wk = wq.shape
+    if wk != K:
         raise ValueError(f"{what}: weight {tuple(wq.shape)} does not match activations {tuple(qx.shape)}")
     if N < 1 or K < 16 or K % 16:
         raise ValueError(f"{what}: N must be at least 1 and K a positive multiple of 16 (N={N}, K={K})")
-    kb, nb = -(-K // _BLK), -(-N // _BLK)
-    if xs.dtype != torch.float32 or xs.shape != (M, kb):
+    kb, nb = (K + 127) // _BLK, (N + 127) // _BLK
+    if xs.dtype is not torch.float32 or xs.shape != (M, kb):
         raise ValueError(f"{what}: xs must be fp32 [{M}, {kb}], got {xs.dtype} {tuple(xs.shape)}")
-    if ws.dtype != torch.float32 or ws.shape != (nb, kb) or (kb > 1 and ws.stride(1) != 1):
+    xs_row, xs_col = xs.stride()
+    ws_row, ws_col = ws.stride() if ws.ndim == 2 else (0, 0)
+    if ws.dtype is not torch.float32 or ws.shape != (nb, kb) or (kb > 1 and ws_col != 1):
         raise ValueError(f"{what}: ws must be fp32 [{nb}, {kb}] with unit column stride, got {ws.dtype} "
                          f"{tuple(ws.shape)}")
-    if len({t.device for t in (qx, wq, xs, ws)}) != 1:
-        raise ValueError(f"{what}: operands are on different devices")
+    ldx, x_col = qx.stride()
+    ldw, w_col = wq.stride()
+    if M <= 1:
+        ldx = K
     if packed:
         if N % 16 or K % _BLK or not wq.is_contiguous():
             raise ValueError(f"{what}: a strip pack is contiguous with N % 16 == 0 and K % 128 == 0")
-    ldx = qx.stride(0) if M > 1 else K
-    ldw = wq.stride(0) if N > 1 else K
-    if qx.stride(1) != 1 or (not packed and wq.stride(1) != 1) or ldx < K or ldw < K or ldx % 16 or ldw % 16:
+        ldw, w_col = K, 1
+    elif N == 1:
+        ldw = K
+    if x_col != 1 or w_col != 1 or ldx < K or ldw < K or ldx % 16 or ldw % 16:
         raise ValueError(f"{what}: rows of qx and wq must be contiguous, their strides multiples of 16")
-    if (M and qx.data_ptr() % 16) or wq.data_ptr() % 16:
+    x_ptr, w_ptr = qx.data_ptr(), wq.data_ptr()
+    if (M and x_ptr % 16) or w_ptr % 16:
         raise ValueError(f"{what}: qx and wq must be 16-byte aligned")
-    args = (qx.data_ptr(), ldx, xs.data_ptr(), xs.stride(0), xs.stride(1), wq.data_ptr(), ldw, int(packed),
-            ws.data_ptr(), ws.stride(0))
-    return args, M, N, K
+    return (x_ptr, ldx, xs.data_ptr(), xs_row, xs_col, w_ptr, ldw, int(packed), ws.data_ptr(), ws_row), M, N, K
 
 
 def fp8_block_gemm(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: torch.Tensor,
@@ -73,9 +81,8 @@ def fp8_block_gemm(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: tor
             raise ValueError(f"fp8_block_gemm: out must be bf16, f16 or f32 [{M}, {N}] on {qx.device} with unit "
                              "column stride and rows that do not overlap")
     if M:
-        with torch.cuda.device(qx.device):
-            rc = _lib.score().b200_fp8_block_gemm(*args, out.data_ptr(), out.stride(0) if M > 1 else N,
-                                                  _DTYPES[out.dtype], M, N, K, _lib.stream_ptr())
-            _lib.check(rc, "b200_fp8_block_gemm")
-            _lib.debug_check_score("b200_fp8_block_gemm")
+        rc = _lib.launch(_lib.score().b200_fp8_block_gemm, qx.device, *args, out.data_ptr(),
+                         out.stride(0) if M > 1 else N, _DTYPES[out.dtype], M, N, K)
+        _lib.check(rc, "b200_fp8_block_gemm")
+        _lib.debug_check_score("b200_fp8_block_gemm")
     return out

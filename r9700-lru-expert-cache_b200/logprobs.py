@@ -35,11 +35,12 @@ class HeadLogprobs(NamedTuple):
 
 
 def _ids(what: str, token_ids: torch.Tensor, M: int, device: torch.device) -> torch.Tensor:
-    _lib.require_cuda(what, token_ids)
-    if token_ids.dtype not in (torch.int64, torch.int32) or token_ids.shape != (M,) or token_ids.device != device:
+    if not token_ids.is_cuda or token_ids.dtype not in (torch.int64, torch.int32) or token_ids.shape != (M,) or token_ids.device != device:
         raise ValueError(f"{what}: token_ids must be int64 or int32 [{M}] on {device}, got {token_ids.dtype} "
                          f"{tuple(token_ids.shape)} on {token_ids.device}")
-    return token_ids.to(torch.int64).contiguous()
+    if token_ids.dtype is not torch.int64 or not token_ids.is_contiguous():
+        token_ids = token_ids.to(torch.int64).contiguous()
+    return token_ids
 
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0) -> TokenLogprobs:
@@ -61,17 +62,15 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
         raise ValueError("token_logprobs: rows of logits must not overlap")
     ids = _ids("token_logprobs", token_ids, M, logits.device)
     dev = logits.device
-    lp, ent, lse = (torch.empty(M, dtype=torch.float32, device=dev) for _ in range(3))
+    lp, ent, lse = torch.empty((3, M), dtype=torch.float32, device=dev).unbind(0)
     rank = torch.empty(M, dtype=torch.int64, device=dev)
-    top_ids = torch.empty(M, top_k, dtype=torch.int64, device=dev)
-    top_lp = torch.empty(M, top_k, dtype=torch.float32, device=dev)
+    top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev)
+    top_lp = torch.empty((M, top_k), dtype=torch.float32, device=dev)
     if M:
-        with torch.cuda.device(dev):
-            rc = _lib.score().b200_token_logprobs(
-                logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0) if M > 1 else V, M, V, ids.data_ptr(),
-                top_k, lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), lse.data_ptr(), top_ids.data_ptr(),
-                top_lp.data_ptr(), _lib.stream_ptr())
-            _lib.check(rc, "b200_token_logprobs")
+        rc = _lib.launch(_lib.score().b200_token_logprobs, dev, logits.data_ptr(), _DTYPES[logits.dtype],
+                         logits.stride(0) if M > 1 else V, M, V, ids.data_ptr(), top_k, lp.data_ptr(), rank.data_ptr(),
+                         ent.data_ptr(), lse.data_ptr(), top_ids.data_ptr(), top_lp.data_ptr())
+        _lib.check(rc, "b200_token_logprobs")
     return TokenLogprobs(lp, ent, lse, rank, top_ids, top_lp)
 
 
@@ -82,15 +81,14 @@ def fp8_head_logprobs(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: 
     args, M, N, K = _operands("fp8_head_logprobs", qx, wq, xs, ws, packed)
     ids = _ids("fp8_head_logprobs", token_ids, M, qx.device)
     dev = qx.device
-    lp, ent, lse = (torch.empty(M, dtype=torch.float32, device=dev) for _ in range(3))
+    lp, ent, lse = torch.empty((3, M), dtype=torch.float32, device=dev).unbind(0)
     if M:
         lib = _lib.score()
-        with torch.cuda.device(dev):
-            scratch = torch.empty(lib.b200_fp8_head_logprobs_workspace_bytes(M, N), dtype=torch.uint8, device=dev)
-            rc = lib.b200_fp8_head_logprobs(*args, ids.data_ptr(), M, N, K, lp.data_ptr(), ent.data_ptr(),
-                                            lse.data_ptr(), scratch.data_ptr(), scratch.numel(), _lib.stream_ptr())
-            _lib.check(rc, "b200_fp8_head_logprobs")
-            _lib.debug_check_score("b200_fp8_head_logprobs")
+        scratch = torch.empty(lib.b200_fp8_head_logprobs_workspace_bytes(M, N), dtype=torch.uint8, device=dev)
+        rc = _lib.launch(lib.b200_fp8_head_logprobs, dev, *args, ids.data_ptr(), M, N, K, lp.data_ptr(),
+                         ent.data_ptr(), lse.data_ptr(), scratch.data_ptr(), scratch.numel())
+        _lib.check(rc, "b200_fp8_head_logprobs")
+        _lib.debug_check_score("b200_fp8_head_logprobs")
     return HeadLogprobs(lp, ent, lse)
 
 
