@@ -591,8 +591,8 @@ struct Operands {
 bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check_operands(const Operands& p) {
-  if (p.M < 0) return -1;
-  if (p.N < 1 || (p.packed && p.N % 16)) return -2;
+  if (p.M < 0 || p.M > (1 << 30)) return -1;         // (coordinates and tile numbers are 32-bit)
+  if (p.N < 1 || p.N > (1 << 30) || (p.packed && p.N % 16)) return -2;
   if (p.K < 16 || p.K % 16 || (p.packed && p.K % 128)) return -3;
   if (p.ldx < p.K || p.ldx % 16 || (!p.packed && (p.ldw < p.K || p.ldw % 16))) return -4;
   if (!aligned(p.x, 16) || !aligned(p.w, 16)) return -10;
@@ -715,23 +715,33 @@ int head_tiles(int N) { return (N + HEAD_BN - 1) / HEAD_BN; }
 
 template <int OUT>
 int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
-  // Columns of a tile and CTAs that split its K: the fewest tile steps on the busiest SM, at the measured
-  // clocks of a 128-K block (320, 540, 900 for 64, 128, 256 columns) and of a cluster's final sum.
-  const int KB = (o.K + 127) / 128, rows = (o.M + BM - 1) / BM, sms = num_sms();
+  // Columns of a tile (256: of a CTA pair's, above 128 rows) and CTAs that split its K, by the time they take: a
+  // start, the busiest SM's 128-K blocks, and with K split the sums' way to their owners, in measured microseconds.
+  // Measured there, chosen first: 5 x 2560 x 2560 at (128, 4) 7.2, (64, 2) 8.0, (64, 1) 9.7; 512 x 1024 x 2560 at
+  // (64, 1) 9.7, (64, 2) 9.9, (128, 4) 12.2; 16 x 10240 x 2560 at (128, 1) 11.9, (64, 1) 16.6; 8192 x 10240 x 2560
+  // at 256 columns 201, (128, 1) 300.
+  const int KB = (o.K + 127) / 128, sms = num_sms();
   int bn = 256, split = 1;
-  double best = 1e30;
-  for (int b = 64; b <= 256; b *= 2)
-    for (int s = 1; s <= (OUT == OUT_STATS || b == 256 ? 1 : 8) && s <= KB; s *= 2) {
-      if (OUT == OUT_STATS && b != HEAD_BN) continue;
-      const long long ctas = (long long)rows * ((o.N + b - 1) / b) * s;
-      if (s > 1 && ctas > sms) continue;
-      const double waves = (double)((ctas + sms - 1) / sms);
-      const double t = waves * ((KB + s - 1) / s) * (b == 64 ? 320. : b == 128 ? 540. : 900.) + (s > 1 ? 2000. : 0.);
-      if (t < best) best = t, bn = b, split = s;
-    }
+  double best = 1e300;
+  auto consider = [&](int b, int s, long long ctas, int at_once, double start, double block) {
+    if (s > KB || (s > 1 && ctas > at_once)) return;
+    const double sums = s > 1 ? 1.2 + std::min(o.M, BM) * (b / 64) * 0.015 : 0.;
+    const double us = start + (double)((ctas + at_once - 1) / at_once) * ((KB + s - 1) / s) * block + sums;
+    if (us < best) best = us, bn = b, split = s;
+  };
+  const long long rows = (o.M + BM - 1) / BM;
+  if (rows > 1)
+    consider(256, 1, (rows + 1) / 2 * ((o.N + 255) / 256), sms / 2, 5.0, 0.56);
+  else
+    consider(256, 1, (o.N + 255) / 256, sms, 5.0, 0.50);
+  for (int s = 1; OUT != OUT_STATS && s <= 8; s *= 2) {
+    consider(128, s, rows * ((o.N + 127) / 128) * s, sms, 4.6, 0.40);
+    consider(64, s, rows * ((o.N + 63) / 64) * s, sms, 3.6, 0.31);
+  }
   if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, 1, stream) : launch<1, 256, OUT>(o, p, 1, stream);
-  if (bn == 128) return launch<1, 128, OUT>(o, p, split, stream);
-  return launch<1, 64, OUT>(o, p, split, stream);
+  if constexpr (OUT != OUT_STATS)
+    return bn == 128 ? launch<1, 128, OUT>(o, p, split, stream) : launch<1, 64, OUT>(o, p, split, stream);
+  return -8;
 }
 
 }  // namespace
