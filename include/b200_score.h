@@ -22,8 +22,9 @@ extern "C" {
  * layout of b200_lmhead.h (N % 16 == 0, K % 128 == 0, ldw unused). y [M, N] with row stride ldy
  * elements. K % 16 == 0, ldx and ldw multiples of 16, 16-byte aligned qx and wq (a TMA copy's rules);
  * a last group of fewer than 128 K and a last block of fewer than 128 rows have scales of their own.
- * Returns 0, -1 M < 0, -2 bad N, -3 bad K, -4 a stride below its row length or not a multiple of 16,
- * -5 bad dtype, -10 misaligned pointer, -12 no tensor map. */
+ * Returns 0, -1 M outside [0, 2^30], -2 bad N (at most 2^30), -3 bad K, -4 a stride below its row length or not a
+ * multiple of 16, -5 bad dtype, -8 more than 2^30 tiles, -10 misaligned pointer, -12 no tensor map, -13 a build
+ * whose register count is not the one the kernels were written for. */
 int b200_fp8_block_gemm(const void* qx, long long ldx, const float* xs, long long xs_row, long long xs_col,
                         const void* wq, long long ldw, int packed, const float* ws, long long ws_row, void* y,
                         long long ldy, int y_dtype, int M, int N, int K, cudaStream_t stream);
@@ -35,7 +36,7 @@ int b200_fp8_block_gemm(const void* qx, long long ldx, const float* xs, long lon
  * top_logprob fp32 [M, top_k]. ids int64 [M]; rank int64 [M]; logprob / entropy / lse fp32 [M].
  * -inf logits have probability 0. A row of nothing but -inf: lse and every logprob -inf, entropy 0.
  * A row with a NaN or +inf: logprob, entropy and lse NaN (NaN comes first among the top ids). An id
- * outside [0, V): logprob NaN, rank 0. Returns 0, -1 M < 0, -2 V < 1, -4 ld < V, -5 bad dtype,
+ * outside [0, V): logprob NaN, rank 0. Returns 0, -1 M outside [0, 2^27], -2 V outside [1, 2^30], -4 ld < V, -5 bad dtype,
  * -6 bad top_k, -10 a pointer that is not a multiple of its element. */
 int b200_token_logprobs(const void* logits, int dtype, long long ld, int M, int V, const long long* ids, int top_k,
                         float* logprob, long long* rank, float* entropy, float* lse, long long* top_ids,

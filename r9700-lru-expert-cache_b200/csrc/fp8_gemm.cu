@@ -4,14 +4,22 @@
 //   y[m, n] = sum_b xs[m, b] ws[n / 128, b] D_b[m, n],   D_b[m, n] = sum_{k in block b} qx[m, k] wq[n, k]
 //
 // Each D_b is one accumulator of the tensor core (fp32, TMEM): 128 tokens x BN weight rows, 128 K. The
-// weight's scale is one number over the tile's 128 rows and the token's is one number per TMEM lane, so a
-// thread that holds a lane's columns needs ONE factor per block: the promotion of D_b into the running sum is
+// weight's scale is one number over 128 rows and the token's is one number per TMEM lane, so a thread that
+// holds a lane's columns needs one factor per block of 128 columns: the promotion of D_b into the running sum is
 // a tcgen05.ld and one fused multiply-add per value, in registers, while the MMAs fill the other accumulators.
 //   warp 0     one lane copies the tiles (tensor maps: zeros beyond M, N and K) into a ring of stages;
 //   warps 1, 3 one lane each issues MMAs, four of K = 32 a 128-K block, into a fresh accumulator;
-//   warp 2     puts the factors xs ws of four 128-K blocks at a time into shared memory;
+//   warp 2     puts the factors xs ws of four 128-K blocks at a time into shared memory (each promoting thread
+//              reading its own row's scales cost more L1 wavefronts than the block's MMAs take);
 //   warps 4-11 two groups of four, each with half of the columns: promote, then write the tile.
 // CTAs (or pairs) walk the tiles, rows first within groups of row tiles, so that tiles in flight share weights.
+//
+// Above 128 rows two CTAs share a tile of 256 rows x 256 columns (cta_group::2): a stage is 32 KB a CTA instead of
+// 48, which the L2 and the shared memory feel. What bounds it (8192 x 10240 x 2560, 201 us, 2130 TFLOP/s; one CTA
+// 216 us): a block's MMAs take 512 clocks, but its accumulators come free only after commit, two waits of 110 to 160
+// clocks, eight TMEM loads with their 64 multiply-adds, and the release to the issuing CTA, about 850 clocks with
+// four accumulators in flight; and the chip's power, which holds the clock near 1.6 GHz. The tensor pipe is active
+// 59 % of the time. A rows' product of few tokens streams the weight: 8 x 151936 x 2560 takes 71 us, 5.5 TB/s.
 #include <algorithm>
 
 #include <cudaTypedefs.h>
@@ -48,7 +56,7 @@ struct Product {
   int box_m;                               // token rows that a stage's copy brings
   int row_tiles, col_tiles;
   int nstage;
-  // op 1
+  // product
   void* y;
   long long ldy;
   int tma_out;                             // y's base and rows are 16-byte aligned
@@ -66,10 +74,10 @@ enum Out { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2, OUT_STATS = 3 };
 // next MMA takes longer than the other one's MMAs.
 template <int BN>
 struct Tile {
-      static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
+  static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
   static constexpr int UN = BN / UNITS;             // their columns
   static constexpr int W = BN / EPI_GROUPS;         // columns of one epilogue group
-  static constexpr int CHUNK = 16;                  // columns of one TMEM load
+  static constexpr int CHUNK = 16;                  // columns of one TMEM load (32: 204 us for 201 above)
   static constexpr int NBUF = 512 / UN > 8 ? 8 : 512 / UN;
   static constexpr int RELEASERS = UNITS == 2 ? EPI_WARPS / 2 : EPI_WARPS;   // warps of a CTA that read one
   static constexpr int BLOCKS = BN > 128 ? BN / 128 : 1;   // weight scales of a tile's 128-K block
@@ -121,7 +129,7 @@ __device__ __forceinline__ int swizzled(int r, int q) {
 // buffers: a tensor-map store that runs on while the warp goes back to its next tile (rows beyond M and columns
 // beyond N are clipped by the copy), or, where y's base or rows are not 16-byte aligned, plain coalesced stores.
 // Straight from registers, 32 rows an instruction, the same tile took 6400 clocks of the 10240 that its MMAs
-// take at K = 2560.
+// take at K = 2560; in boxes of 64 bytes the product above takes 215 us instead of 208.
 template <int OUT, int W, bool SEG>
 __device__ __forceinline__ void store_rows(const Product& p, const CUtensorMap* ymap, char* bufs, int& turn, int m0,
                                            int n0, int lane, const float2 (&acc)[W / 2]) {

@@ -250,5 +250,11 @@ class Fp8TargetHead:
         self.n_fp8 += 1
         return y.reshape(*x.shape[:-1], y.shape[-1])
 
+    def score(self, hidden: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0):
+        """The log probabilities of a prompt's tokens under this head (``logprobs.score_prompt``):
+        hidden [M, K] for any M, token_ids [M], with ``top_k`` alternatives of every row."""
+        from .logprobs import score_prompt
+        return score_prompt(hidden, self.wq, self.ws, token_ids, top_k=top_k)
+
     def __getattr__(self, name):        # everything else passes through to the original
         return getattr(self.orig, name)

@@ -319,3 +319,23 @@ def test_score_prompt(cuda, M, rows):
     assert (b.top_ids[:, 0] == y.bfloat16().float().argmax(1)).float().mean() > 0.9 and b.top_ids.shape == (M, 6)
     with pytest.raises(ValueError):
         LP.score_prompt(hidden, wq, ws, ids, top_k=2, rows_at_once=0)
+
+
+def test_target_head_scores_its_prompt(cuda):
+    """Fp8TargetHead.score is score_prompt on the head's own pack; a scoring product above the decode path's
+    64 rows agrees with the decode path's logits row for row."""
+    N, K, M = 2048, 256, 90
+    g = torch.Generator(device=cuda).manual_seed(5)
+    w = (torch.randn(N, K, device=cuda, generator=g) * 0.1).bfloat16()
+    head = P.fp8_target_lmhead.Fp8TargetHead(None, w)
+    hidden = torch.randn(M, K, device=cuda, generator=g).bfloat16()
+    ids = torch.randint(N, (M,), device=cuda, generator=g)
+    a, b = head.score(hidden, ids), LP.score_prompt(hidden, head.wq, head.ws, ids)
+    for u, v in zip(a, b):
+        assert torch.equal(u, v)
+    qx, xs = P.fused_silu_mul_quant.per_token_group_quant_fp8(hidden)
+    y = P.fp8_block_gemm.fp8_block_gemm(qx, head.wq, xs, head.ws, packed=True)
+    decode = torch.cat([P.fp8_target_lmhead.gemm_fp8_block(hidden[i:i + 30].contiguous(), head.wq, head.ws)
+                        for i in range(0, M, 30)])
+    # both round the same fp32 sums, added in another order, to bf16: at most one step apart
+    assert ((y.float() - decode.float()).abs() <= 2.0 ** -7 * decode.float().abs() + 1e-5).all()

@@ -35,7 +35,7 @@ def _gemm(M=4, N=128, K=128, ldx=None, ldw=None, ldy=None, packed=0, dtype=0, x=
 
 
 @pytest.mark.parametrize("args,code", [
-    (dict(M=-1), -1), (dict(N=0), -2), (dict(N=130, packed=1), -2), (dict(K=0), -3), (dict(K=24), -3),
+    (dict(M=-1), -1), (dict(M=(1 << 30) + 1), -1), (dict(N=0), -2), (dict(N=(1 << 30) + 1, ldy=1 << 31), -2), (dict(N=130, packed=1), -2), (dict(K=0), -3), (dict(K=24), -3),
     (dict(K=144, packed=1), -3), (dict(ldx=112), -4), (dict(ldx=136), -4), (dict(ldw=112), -4), (dict(ldw=130), -4),
     (dict(ldy=127), -4), (dict(dtype=3), -5), (dict(dtype=-1), -5), (dict(x=8), -10), (dict(w=17), -10),
     (dict(y=17), -10), (dict(y=18, dtype=2), -10), (dict(M=0), 0)])
@@ -49,7 +49,7 @@ def _logprobs(dtype=0, ld=100, M=4, V=100, top_k=0, x=16):
 
 
 @pytest.mark.parametrize("args,code", [
-    (dict(M=-1), -1), (dict(V=0), -2), (dict(ld=99), -4), (dict(dtype=3), -5), (dict(top_k=-1), -6),
+    (dict(M=-1), -1), (dict(M=(1 << 27) + 1), -1), (dict(V=0), -2), (dict(V=(1 << 30) + 1, ld=1 << 31), -2), (dict(ld=99), -4), (dict(dtype=3), -5), (dict(top_k=-1), -6),
     (dict(top_k=65), -6), (dict(V=10, top_k=11), -6), (dict(x=17), -10), (dict(x=18, dtype=2), -10), (dict(M=0), 0)])
 def test_logprobs_codes(args, code):
     assert _logprobs(**args) == code
