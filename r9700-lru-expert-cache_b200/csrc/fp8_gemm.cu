@@ -202,24 +202,35 @@ __device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, f
     }
     if (mine) p.token[m] = __uint_as_float(bits);
   }
+  // y = (x - m) log2 e as one fused multiply-add, x log2 e - R with R = m log2 e rounded; the sums are moved from R
+  // to m at the end. (A multiplication and a subtraction each, scalar, took 1640 us for 1540 at 4096 x 151936 x 2560.)
   LogitStat st;
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-  for (int c = 0; c < W / 2; ++c) mx[c & 3] = fmaxf(mx[c & 3], fmaxf(acc[c].x, acc[c].y));
+  for (int c = 0; c < W / 2; ++c) mx[c & 3] = max3(mx[c & 3], acc[c].x, acc[c].y);
   st.m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
   const float ref = st.m == -INFINITY ? 0.f : st.m;
-  float s[2] = {}, w[2] = {};
+  float moved = ref * LOG2E, rest = fmaf(ref, LOG2E, -moved);
+  if (!(fabsf(ref) < LARGE)) {                       // there R is too coarse
+    const float2 by = make_float2(-ref, -ref);
+#pragma unroll
+    for (int c = 0; c < W / 2; ++c) acc[c] = add2(acc[c], by);
+    moved = rest = 0.f;
+  }
+  const float2 l2 = make_float2(LOG2E, LOG2E), r2 = make_float2(-moved, -moved);
+  float2 s[2] = {}, w[2] = {};
 #pragma unroll
   for (int c = 0; c < W / 2; ++c) {
-    const float dx = max_nan(acc[c].x - ref, -200.f), dy = max_nan(acc[c].y - ref, -200.f);  // e^-200 = 0 in fp32
-    const float ex = __expf(dx), ey = __expf(dy);
-    s[0] += ex;
-    s[1] += ey;
-    w[0] = fmaf(ex, dx, w[0]);
-    w[1] = fmaf(ey, dy, w[1]);
+    float2 y = fma2(acc[c], l2, r2);
+    y = make_float2(max_nan(y.x, LOWEST_Y), max_nan(y.y, LOWEST_Y));
+    const float2 x = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+    s[c & 1] = add2(s[c & 1], x);
+    w[c & 1] = fma2(x, y, w[c & 1]);
   }
-  st.s = s[0] + s[1];
-  st.w = w[0] + w[1];
+  const float total = (s[0].x + s[0].y) + (s[1].x + s[1].y), weighted = (w[0].x + w[0].y) + (w[1].x + w[1].y);
+  const float back = exp2_approx(-rest);
+  st.s = total * back;
+  st.w = fmaf(-rest, total, weighted) * back * LN2;
   if (isnan(st.s)) st = LogitStat{0.f, NAN, NAN};    // a NaN, or +inf (whose difference from itself is NaN)
   return st;
 }

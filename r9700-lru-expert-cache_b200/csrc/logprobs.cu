@@ -30,18 +30,11 @@ namespace {
 
 using namespace b200;
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr int BIG = 256, SMALL = 64;        // threads of a CTA for long and for short rows
 constexpr int MAX_TOP = 64;
 constexpr int MAX_CLUSTER = 8;
 constexpr int INFLIGHT = 2;                // chunks a thread loads at a time
 constexpr float HEADROOM = 58.f;           // 2^58 times the vocabulary stays far below fp32's largest
-// Beyond this size a logit times log2 e is known to no better than a few units, or out of fp32's range: below
-// -LARGE a logit is not taken as a reference (beside any other it has no weight), and a row whose largest logit is
-// not within +-LARGE is done again in natural units.
-constexpr float LARGE = 4e7f;
-constexpr float LOWEST_Y = -160.f;         // 2^-160 = 0 in fp32, and 0 * -160 = 0 where 0 * -inf is not
-
 struct Raw {                               // 32 bytes of logits
   uint32_t w[8];
 };
@@ -125,29 +118,6 @@ __device__ __forceinline__ Raw ld_stream(const void* p) {
                  "=r"(r.w[7])
                : "l"(p));
   return r;
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// (a.x + b.x, a.y + b.y) and a fused multiply-add, one packed instruction each.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-  return *reinterpret_cast<float2*>(&r);
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
-      : "=l"(r)
-      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
-        "l"(*reinterpret_cast<unsigned long long*>(&c)));
-  return *reinterpret_cast<float2*>(&r);
 }
 
 // Sums relative to `from` made relative to `to` >= from. A part without logits above -inf has no reference.

@@ -16,6 +16,43 @@ B200_DEVINL float max_nan(float a, float b) {
   return r;
 }
 
+B200_DEVINL float max3(float a, float b, float c) {   // ignores NaN
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// Beyond this size a logit times log2 e is known to no better than a few units, or out of fp32's range: below
+// -LARGE a logit is not taken as a reference (beside any other it has no weight), and a row whose largest logit is
+// not within +-LARGE is done again in natural units.
+constexpr float LARGE = 4e7f;
+constexpr float LOWEST_Y = -160.f;         // 2^-160 = 0 in fp32, and 0 * -160 = 0 where 0 * -inf is not
+
+B200_DEVINL float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// (a.x + b.x, a.y + b.y) and a fused multiply-add, one packed instruction each.
+B200_DEVINL float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+  return *reinterpret_cast<float2*>(&r);
+}
+B200_DEVINL float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(r)
+      : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)),
+        "l"(*reinterpret_cast<unsigned long long*>(&c)));
+  return *reinterpret_cast<float2*>(&r);
+}
+
 // Statistics of a row of logits relative to a reference m (its running maximum):
 // s = sum e^(x - m), w = sum e^(x - m) (x - m). m = -inf: nothing but -inf so far, s = w = 0.
 struct LogitStat {
