@@ -134,15 +134,20 @@ def stream_ptr(stream=None) -> c_vp:
     return c_vp(s.cuda_stream)
 
 
-def launch(fn, device, *args) -> int:
-    """fn(*args, stream) on the current stream of `device`, with `device` current. (The raw stream
-    handle: building a torch.cuda.Stream for it costs as much as the launch.)"""
+def launch(what: str, fn, device, *args) -> None:
+    """fn(*args, stream) on the current stream of `device`, with `device` current; raises on an error
+    code. (The raw stream handle: building a torch.cuda.Stream for it costs as much as the launch.)"""
     import torch
     index = device.index
-    if index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
+    if _CHECK:
+        debug_check_score(what)
 
 
 def check(rc: int, what: str) -> None:

@@ -70,19 +70,22 @@ def fp8_block_gemm(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: tor
     wq may be strided by multiples of 16. Each 128-K block's sum is scaled and added in fp32 and
     the result rounded once."""
     args, M, N, K = _operands("fp8_block_gemm", qx, wq, xs, ws, packed)
+    ldy = N
     if out is None:
-        if out_dtype not in _DTYPES:
+        code = _DTYPES.get(out_dtype)
+        if code is None:
             raise ValueError(f"fp8_block_gemm: unsupported output dtype {out_dtype}")
         out = torch.empty(M, N, dtype=out_dtype, device=qx.device)
     else:
         _lib.require_cuda("fp8_block_gemm", out)
-        if out.shape != (M, N) or out.dtype not in _DTYPES or out.device != qx.device or \
+        code = _DTYPES.get(out.dtype)
+        if out.shape != (M, N) or code is None or out.device != qx.device or \
                 (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"fp8_block_gemm: out must be bf16, f16 or f32 [{M}, {N}] on {qx.device} with unit "
                              "column stride and rows that do not overlap")
+        if M > 1:
+            ldy = out.stride(0)
     if M:
-        rc = _lib.launch(_lib.score().b200_fp8_block_gemm, qx.device, *args, out.data_ptr(),
-                         out.stride(0) if M > 1 else N, _DTYPES[out.dtype], M, N, K)
-        _lib.check(rc, "b200_fp8_block_gemm")
-        _lib.debug_check_score("b200_fp8_block_gemm")
+        _lib.launch("b200_fp8_block_gemm", _lib.score().b200_fp8_block_gemm, qx.device, *args, out.data_ptr(), ldy, code,
+                    M, N, K)
     return out

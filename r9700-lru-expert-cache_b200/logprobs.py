@@ -35,7 +35,7 @@ class HeadLogprobs(NamedTuple):
 
 
 def _ids(what: str, token_ids: torch.Tensor, M: int, device: torch.device) -> torch.Tensor:
-    if not token_ids.is_cuda or token_ids.dtype not in (torch.int64, torch.int32) or token_ids.shape != (M,) or token_ids.device != device:
+    if token_ids.device != device or token_ids.shape != (M,) or token_ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: token_ids must be int64 or int32 [{M}] on {device}, got {token_ids.dtype} "
                          f"{tuple(token_ids.shape)} on {token_ids.device}")
     if token_ids.dtype is not torch.int64 or not token_ids.is_contiguous():
@@ -51,26 +51,29 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     A -inf logit has probability 0. A row of nothing but -inf has logsumexp and log probabilities
     -inf and entropy 0; a row with a NaN or +inf has NaN for all three. A token id outside [0, V)
     has log probability NaN and rank 0."""
-    _lib.require_cuda("token_logprobs", logits)
-    if logits.ndim != 2 or logits.dtype not in _DTYPES or logits.shape[1] < 1 or \
-            (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError("token_logprobs: logits must be bf16, f16 or f32 [M, V] with unit column stride")
+    dev, code = logits.device, _DTYPES.get(logits.dtype)
+    if not logits.is_cuda or code is None or logits.ndim != 2:
+        _lib.require_cuda("token_logprobs", logits)
+        raise ValueError("token_logprobs: logits must be bf16, f16 or f32 [M, V]")
     M, V = logits.shape
-    if not 0 <= top_k <= min(V, MAX_TOP_K):
+    ld, col = logits.stride()
+    if V < 1 or (V > 1 and col != 1):
+        raise ValueError("token_logprobs: logits must have columns, of unit stride")
+    if not 0 <= top_k <= MAX_TOP_K or top_k > V:
         raise ValueError(f"token_logprobs: top_k must be between 0 and min(V, {MAX_TOP_K}), got {top_k}")
-    if M > 1 and logits.stride(0) < V:
+    if M <= 1:
+        ld = V
+    elif ld < V:
         raise ValueError("token_logprobs: rows of logits must not overlap")
-    ids = _ids("token_logprobs", token_ids, M, logits.device)
-    dev = logits.device
-    lp, ent, lse = torch.empty((3, M), dtype=torch.float32, device=dev).unbind(0)
+    ids = _ids("token_logprobs", token_ids, M, dev)
+    lp, ent, lse = torch.empty(3, M, dtype=torch.float32, device=dev).unbind(0)
     rank = torch.empty(M, dtype=torch.int64, device=dev)
-    top_ids = torch.empty((M, top_k), dtype=torch.int64, device=dev)
-    top_lp = torch.empty((M, top_k), dtype=torch.float32, device=dev)
+    top_ids = torch.empty(M, top_k, dtype=torch.int64, device=dev)
+    top_lp = torch.empty(M, top_k, dtype=torch.float32, device=dev)
     if M:
-        rc = _lib.launch(_lib.score().b200_token_logprobs, dev, logits.data_ptr(), _DTYPES[logits.dtype],
-                         logits.stride(0) if M > 1 else V, M, V, ids.data_ptr(), top_k, lp.data_ptr(), rank.data_ptr(),
-                         ent.data_ptr(), lse.data_ptr(), top_ids.data_ptr(), top_lp.data_ptr())
-        _lib.check(rc, "b200_token_logprobs")
+        _lib.launch("b200_token_logprobs", _lib.score().b200_token_logprobs, dev, logits.data_ptr(), code, ld, M, V,
+                    ids.data_ptr(), top_k, lp.data_ptr(), rank.data_ptr(), ent.data_ptr(), lse.data_ptr(),
+                    top_ids.data_ptr(), top_lp.data_ptr())
     return TokenLogprobs(lp, ent, lse, rank, top_ids, top_lp)
 
 
@@ -81,14 +84,12 @@ def fp8_head_logprobs(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: 
     args, M, N, K = _operands("fp8_head_logprobs", qx, wq, xs, ws, packed)
     ids = _ids("fp8_head_logprobs", token_ids, M, qx.device)
     dev = qx.device
-    lp, ent, lse = torch.empty((3, M), dtype=torch.float32, device=dev).unbind(0)
+    lp, ent, lse = torch.empty(3, M, dtype=torch.float32, device=dev).unbind(0)
     if M:
         lib = _lib.score()
         scratch = torch.empty(lib.b200_fp8_head_logprobs_workspace_bytes(M, N), dtype=torch.uint8, device=dev)
-        rc = _lib.launch(lib.b200_fp8_head_logprobs, dev, *args, ids.data_ptr(), M, N, K, lp.data_ptr(),
-                         ent.data_ptr(), lse.data_ptr(), scratch.data_ptr(), scratch.numel())
-        _lib.check(rc, "b200_fp8_head_logprobs")
-        _lib.debug_check_score("b200_fp8_head_logprobs")
+        _lib.launch("b200_fp8_head_logprobs", lib.b200_fp8_head_logprobs, dev, *args, ids.data_ptr(), M, N, K,
+                    lp.data_ptr(), ent.data_ptr(), lse.data_ptr(), scratch.data_ptr(), scratch.numel())
     return HeadLogprobs(lp, ent, lse)
 
 
