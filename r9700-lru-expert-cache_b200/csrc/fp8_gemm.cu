@@ -694,8 +694,10 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   if (rc != 0) return rc;
   const int tiles = p.row_tiles * p.col_tiles, KB = (o.K + 127) / 128;
   const int cl = CG == 2 ? 2 : split;
-  const int clusters = cl == 1 || CG == 2 ? std::min(tiles, num_sms() / cl) : tiles;
-  const int per_cta = CG == 2 || split == 1 ? (tiles + clusters - 1) / clusters * KB : (KB + split - 1) / split;
+  // As few CTAs (pairs) as take no more turns than all SMs would.
+  const int turns = split > 1 ? 1 : (tiles + num_sms() / cl - 1) / (num_sms() / cl);
+  const int clusters = (tiles + turns - 1) / turns;
+  const int per_cta = split > 1 ? (KB + split - 1) / split : turns * KB;
   p.nstage = std::min({MAX_STAGES, (SMEM_CAP - 1024 - ring_offset<OUT>()) / STAGE, std::max(2, per_cta)});
   int smem = std::max(SMEM_MIN, 1024 + ring_offset<OUT>() + p.nstage * STAGE);
   auto kern = product_kernel<CG, BN, OUT>;
