@@ -19,7 +19,7 @@
 // 216 us): a block's MMAs take 512 clocks, but its accumulators come free only after commit, two waits of 110 to 160
 // clocks, eight TMEM loads with their 64 multiply-adds, and the release to the issuing CTA, about 850 clocks with
 // four accumulators in flight; and the chip's power, which holds the clock near 1.6 GHz. The tensor pipe is active
-// 59 % of the time. A rows' product of few tokens streams the weight: 8 x 151936 x 2560 takes 71 us, 5.5 TB/s.
+// 59 % of the time. Few tokens stream the weight: 8 x 151936 x 2560 takes 67 us, 5.8 TB/s.
 #include <algorithm>
 
 #include <cudaTypedefs.h>
@@ -56,6 +56,7 @@ struct Product {
   int box_m;                               // token rows that a stage's copy brings
   int row_tiles, col_tiles;
   int nstage;
+  int quarters, a_bytes;                   // quarters of 32 rows with tokens; bytes of a stage's token rows (CG = 1)
   // product
   void* y;
   long long ldy;
@@ -235,11 +236,14 @@ __device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, f
   return st;
 }
 
-// Shared memory: barriers | factors [2][FGROUP][F_LD] | output buffers or statistics | ring of stages.
+// Shared memory: barriers | factors | output buffers or statistics | ring of stages, each the token rows and the
+// weight rows. Where one row tile holds all tokens (few), only the quarters of 32 rows that hold some have output
+// buffers and a stage holds only those rows, which leaves more stages for the weight (8 rows: 6 for 4, 67 us for 73 at 8 x 151936 x 2560); the MMAs then
+// read on past them, into rows of the accumulator that nobody looks at.
 __host__ __device__ constexpr int out_offset() { return (1024 + 2 * FGROUP * F_LD * 4 + 1023) / 1024 * 1024; }
 template <int OUT>
-__host__ __device__ constexpr int ring_offset() {
-  return out_offset() + (OUT == OUT_STATS ? 2 * 3 * EPI_GROUPS * BM * 4 : EPI_WARPS * OUT_BUFS * OUT_BUF);
+__host__ __device__ constexpr int ring_offset(int quarters) {
+  return out_offset() + (OUT == OUT_STATS ? 2 * 3 * EPI_GROUPS * BM * 4 : EPI_GROUPS * quarters * OUT_BUFS * OUT_BUF);
 }
 
 // One CTA (CG = 1; gridDim / cluster size clusters, whose CTAs split K) or one CTA pair (CG = 2).
@@ -250,7 +254,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   constexpr int W = Tile<BN>::W, NBUF = Tile<BN>::NBUF, UNITS = Tile<BN>::UNITS, UN = Tile<BN>::UN;
   constexpr bool SEG = CG == 2 && UNITS == 2;                      // a group's columns: 64 of each 128-column block
   constexpr int B_ROWS = BN / CG;                    // weight rows in this CTA's shared memory
-  constexpr int STAGE = (BM + B_ROWS) * 128;
+  const int quarters = CG == 1 ? p.quarters : 4, A_BYTES = CG == 1 ? p.a_bytes : BM * 128;
+  const int STAGE = A_BYTES + B_ROWS * 128;
   constexpr bool CAN_SPLIT = CG == 1 && OUT != OUT_STATS && !Tile<BN>::SPLIT_REGS;
   extern __shared__ char sm_raw[];
   char* sm = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
@@ -264,7 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 2);
   float* factors = reinterpret_cast<float*>(sm + 1024);
   float* stat_s = reinterpret_cast<float*>(sm + out_offset());      // head: [2][3][EPI_GROUPS][BM]
-  char* ring = sm + ring_offset<OUT>();
+  char* ring = sm + ring_offset<OUT>(quarters);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = cluster_rank(), csize = cluster_size();
   const uint32_t split = CAN_SPLIT ? csize : 1, part = CAN_SPLIT ? crank : 0;
@@ -295,9 +300,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t dst = smem_u32(ring + at.s * STAGE);
     tma_load_2d<CG>(dst, &xmap, at.kb * 128, at.m, bar);
     if (p.packed)
-      tma_load_4d<CG>(dst + BM * 128, &wmap, 0, 0, at.n / 16, at.kb, bar);
+      tma_load_4d<CG>(dst + A_BYTES, &wmap, 0, 0, at.n / 16, at.kb, bar);
     else
-      tma_load_2d<CG>(dst + BM * 128, &wmap, at.kb * 128, at.n, bar);
+      tma_load_2d<CG>(dst + A_BYTES, &wmap, at.kb * 128, at.n, bar);
     ++at.count;
     if (++at.s == nstage) at.s = 0, ++at.round;
     if (++at.kb == kb1) {
@@ -384,7 +389,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t st = smem_u32(ring + s * STAGE);
-          const uint64_t a = sw128_desc(st), b = sw128_desc(st + BM * 128 + b_offset);
+          const uint64_t a = sw128_desc(st), b = sw128_desc(st + A_BYTES + b_offset);
           const uint32_t d = tmem + buf * UN;
 #pragma unroll
           for (int k = 0; k < 4; ++k) tc_mma_f8<CG>(d, a + 2 * k, b + 2 * k, idesc, k > 0 ? 1u : 0u);
@@ -502,7 +507,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         ++turn;
       } else if (ok && split == 1 && n < p.N && m - lane < p.M) {
-        store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (warp - 4) * OUT_BUFS * OUT_BUF, turn, m - lane, n, lane, acc);
+        store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (group * quarters + quarter) * OUT_BUFS * OUT_BUF, turn,
+                                m - lane, n, lane, acc);
       }
     }
     if (OUT != OUT_STATS && lane == 0) bulk_wait_all();
@@ -516,8 +522,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     // nothing else uses here, and it adds them in rank order.
     if (split > 1) {
       const int share = BN / split;
-      float* sums = reinterpret_cast<float*>(sm + out_offset());       // [split][BM][share]
-      static_assert(BM * BN * 4 <= EPI_WARPS * OUT_BUFS * OUT_BUF, "the output buffers hold a tile");
+      float* sums = reinterpret_cast<float*>(sm + out_offset());       // [split][32 quarters][share]
+      static_assert(32 * BN * 4 <= EPI_GROUPS * OUT_BUFS * OUT_BUF, "the output buffers hold a tile");
+      const int cap = 32 * quarters;
       int rt, ct;
       tile_at(p, first, rt, ct);
       const int rows = min(BM, p.M - rt * BM);
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int c = 0; c < W; c += 4) {
             const int col = group * W + c, owner = col / share;
-            st_cluster_f4(map_to_rank(smem_u32(sums + (part * BM + r) * share + col - owner * share), owner),
+            st_cluster_f4(map_to_rank(smem_u32(sums + (part * cap + r) * share + col - owner * share), owner),
                           make_float4(acc[c / 2].x, acc[c / 2].y, acc[c / 2 + 1].x, acc[c / 2 + 1].y));
           }
         }
@@ -539,7 +546,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int r = e / quads, c = (e - r * quads) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (uint32_t q = 0; q < split; ++q) {
-          const float4 u = *reinterpret_cast<const float4*>(sums + (q * BM + r) * share + c);
+          const float4 u = *reinterpret_cast<const float4*>(sums + (q * cap + r) * share + c);
           v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
         }
         const int n = ct * BN + part * share + c;
@@ -679,7 +686,7 @@ int num_sms() {
 
 template <int CG, int BN, int OUT>
 int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
-  constexpr int B_ROWS = BN / CG, STAGE = (BM + B_ROWS) * 128;
+  constexpr int B_ROWS = BN / CG;
   p.xs = o.xs, p.xs_row = o.xs_row, p.xs_col = o.xs_col, p.ws = o.ws, p.ws_row = o.ws_row;
   p.M = o.M, p.N = o.N, p.K = o.K, p.packed = o.packed;
   p.box_m = std::min(BM, (o.M + 7) / 8 * 8);
@@ -694,12 +701,18 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   if (rc != 0) return rc;
   const int tiles = p.row_tiles * p.col_tiles, KB = (o.K + 127) / 128;
   const int cl = CG == 2 ? 2 : split;
-  // As few CTAs (pairs) as take no more turns than all SMs would.
+  // As few CTAs (pairs) as take no more turns than all SMs would: 8 x 151936 x 2560, whose 594 tiles are four turns and
+  // two tiles of 148 SMs, takes 73 us on 119 and 76 on 148.
   const int turns = split > 1 ? 1 : (tiles + num_sms() / cl - 1) / (num_sms() / cl);
   const int clusters = (tiles + turns - 1) / turns;
   const int per_cta = split > 1 ? (KB + split - 1) / split : turns * KB;
-  p.nstage = std::min({MAX_STAGES, (SMEM_CAP - 1024 - ring_offset<OUT>()) / STAGE, std::max(2, per_cta)});
-  int smem = std::max(SMEM_MIN, 1024 + ring_offset<OUT>() + p.nstage * STAGE);
+  const bool few = CG == 1 && p.row_tiles == 1;
+  p.quarters = few ? (o.M + 31) / 32 : 4;
+  p.a_bytes = few ? p.box_m * 128 : BM * 128;
+  const int stage = p.a_bytes + B_ROWS * 128;
+  const int fixed = 1024 + ring_offset<OUT>(p.quarters) + (BM * 128 - p.a_bytes);   // alignment, all before the ring, reads past it
+  p.nstage = std::min({MAX_STAGES, (SMEM_CAP - fixed) / stage, std::max(2, per_cta)});
+  const int smem = std::max(SMEM_MIN, fixed + p.nstage * stage);
   auto kern = product_kernel<CG, BN, OUT>;
   static bool ready[MAX_DEVICES] = {};
   int dev = 0;
