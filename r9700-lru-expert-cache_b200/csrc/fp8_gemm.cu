@@ -78,7 +78,6 @@ struct Tile {
   static constexpr int UNITS = BN == 256 ? 2 : 1;   // accumulators of a 128-K block
   static constexpr int UN = BN / UNITS;             // their columns
   static constexpr int W = BN / EPI_GROUPS;         // columns of one epilogue group
-  static constexpr int CHUNK = 16;                  // columns of one TMEM load (32: 204 us for 201 above)
   static constexpr int NBUF = 512 / UN > 8 ? 8 : 512 / UN;
   static constexpr int RELEASERS = UNITS == 2 ? EPI_WARPS / 2 : EPI_WARPS;   // warps of a CTA that read one
   static constexpr int BLOCKS = BN > 128 ? BN / 128 : 1;   // weight scales of a tile's 128-K block
@@ -468,12 +467,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float* now = my_factors + ((fg & 1) * FGROUP + fi) * F_LD;
         const float scale0 = now[0], scale1 = SEG ? now[BM] : scale0;
         const uint32_t src = lanes + buf * UN;
-        constexpr int C = Tile<BN>::CHUNK;
+        constexpr int C = 16;                        // columns of one TMEM load (32: 204 us for 201 above)
 #pragma unroll
         for (int c = 0; c < W; c += C) {
           uint32_t v[C];
-          tmem_ld<C>(src + c, v);
-          tmem_wait_ld<C>(v);
+          tmem_ld16(src + c, v);
+          tmem_wait_ld16(v);
           if (c + C == W) {
             tc_fence_before();
             __syncwarp();

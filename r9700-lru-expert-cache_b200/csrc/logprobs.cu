@@ -30,7 +30,7 @@ namespace {
 
 using namespace b200;
 
-constexpr int BIG = 256, SMALL = 64;        // threads of a CTA for long and for short rows
+constexpr int BIG = 256, MID = 128, SMALL = 64;   // threads of a CTA for long, ordinary and short rows
 constexpr int MAX_TOP = 64;
 constexpr int MAX_CLUSTER = 8;
 constexpr int INFLIGHT = 2;                // chunks a thread loads at a time
@@ -495,21 +495,24 @@ int launch_t(const Args& p, int M, int cluster, cudaStream_t stream) {
 
 template <typename T>
 int launch(const Args& p, int M, cudaStream_t stream) {
-  // Small CTAs for rows of up to 16 chunks a thread of those, where a large one would mostly synchronise.
+  // CTAs of few threads for short rows, which mostly synchronise: up to 1024 chunks, and with many rows up to 4096
+  // (777 x 50001 f16 with 8 alternatives 26.5 us in 128 threads and 28.0 in 256, 2000 x 20000 bf16 30.2 and 36.4, but
+  // 16 x 32000 9.1 and 8.2, and 4096 x 151936 with 20 alternatives 494 and 258: a top logit's thread has more chunks
+  // to read again. One warp a row took 142 us for 32 at 4096 x 2000 with 20.)
   const long long chunks = (long long)p.V / Chunk<T>::N + 1;
-  const bool small = chunks <= 1024;
-  const int threads = small ? SMALL : BIG;
+  const int threads = chunks <= 1024 ? SMALL : chunks <= 4096 && M >= num_sms() ? MID : BIG;
   // CTAs a row, each with two chunks a thread at least: the fewest turns of the SMs' CTAs, a turn being a CTA's
-  // share of the row at its share of the bandwidth (10 GB/s) and about 8 us of reduction.
-  const long long slots = (long long)(1024 / BIG) * num_sms();
-  const double row_us = (double)p.V * sizeof(T) * 1e-4;
+  // share of the row at its share of the bandwidth and about 8 us of reduction.
+  const long long slots = (long long)(1024 / threads) * num_sms();
+  const double row_us = (double)p.V * sizeof(T) * slots / 5.9e6;
   int cluster = 1;
   double best = 1e300;
   for (int c = 1; c <= MAX_CLUSTER && (c == 1 || chunks / c >= 2 * threads); c *= 2) {
     const double us = (double)((M * (long long)c + slots - 1) / slots) * (row_us / c + 8.);
     if (us < best) best = us, cluster = c;
   }
-  return small ? launch_t<T, SMALL>(p, M, cluster, stream) : launch_t<T, BIG>(p, M, cluster, stream);
+  return threads == SMALL ? launch_t<T, SMALL>(p, M, cluster, stream)
+                          : threads == MID ? launch_t<T, MID>(p, M, cluster, stream) : launch_t<T, BIG>(p, M, cluster, stream);
 }
 
 }  // namespace
