@@ -237,8 +237,8 @@ __device__ __forceinline__ LogitStat row_stats(const Product& p, int m, int n, f
 
 // Shared memory: barriers | factors | output buffers or statistics | ring of stages, each the token rows and the
 // weight rows. Where one row tile holds all tokens (few), only the quarters of 32 rows that hold some have output
-// buffers and a stage holds only those rows, which leaves more stages for the weight (8 rows: 6 for 4, 67 us for 73 at 8 x 151936 x 2560); the MMAs then
-// read on past them, into rows of the accumulator that nobody looks at.
+// buffers and a stage holds only those rows, which leaves more stages for the weight (8 rows: 6 for 4, 67 us for 73
+// at 8 x 151936 x 2560); the MMAs then read on past them, into rows of the accumulator that nobody looks at.
 __host__ __device__ constexpr int out_offset() { return (1024 + 2 * FGROUP * F_LD * 4 + 1023) / 1024 * 1024; }
 template <int OUT>
 __host__ __device__ constexpr int ring_offset(int quarters) {
@@ -668,8 +668,8 @@ int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es
   const auto fn = encoder();
   if (fn == nullptr) return -12;
   return fn(m, es == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box,
-            one, CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
+            one, CU_TENSOR_MAP_INTERLEAVE_NONE, row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
 }
 
 constexpr int MAX_DEVICES = 64;
@@ -709,7 +709,8 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   p.quarters = few ? (o.M + 31) / 32 : 4;
   p.a_bytes = few ? p.box_m * 128 : BM * 128;
   const int stage = p.a_bytes + B_ROWS * 128;
-  const int fixed = 1024 + ring_offset<OUT>(p.quarters) + (BM * 128 - p.a_bytes);   // alignment, all before the ring, reads past it
+  // alignment, all before the ring, what the MMAs read past its end
+  const int fixed = 1024 + ring_offset<OUT>(p.quarters) + (BM * 128 - p.a_bytes);
   p.nstage = std::min({MAX_STAGES, (SMEM_CAP - fixed) / stage, std::max(2, per_cta)});
   const int smem = std::max(SMEM_MIN, fixed + p.nstage * stage);
   auto kern = product_kernel<CG, BN, OUT>;

@@ -512,7 +512,8 @@ int launch(const Args& p, int M, cudaStream_t stream) {
     if (us < best) best = us, cluster = c;
   }
   return threads == SMALL ? launch_t<T, SMALL>(p, M, cluster, stream)
-                          : threads == MID ? launch_t<T, MID>(p, M, cluster, stream) : launch_t<T, BIG>(p, M, cluster, stream);
+                          : threads == MID ? launch_t<T, MID>(p, M, cluster, stream)
+                                           : launch_t<T, BIG>(p, M, cluster, stream);
 }
 
 }  // namespace

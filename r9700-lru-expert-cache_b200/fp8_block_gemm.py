@@ -86,6 +86,6 @@ def fp8_block_gemm(qx: torch.Tensor, wq: torch.Tensor, xs: torch.Tensor, ws: tor
         if M > 1:
             ldy = out.stride(0)
     if M:
-        _lib.launch("b200_fp8_block_gemm", _lib.score().b200_fp8_block_gemm, qx.device, *args, out.data_ptr(), ldy, code,
-                    M, N, K)
+        _lib.launch("b200_fp8_block_gemm", _lib.score().b200_fp8_block_gemm, qx.device, *args, out.data_ptr(), ldy,
+                    code, M, N, K)
     return out
