@@ -184,3 +184,39 @@ def test_refusals(cuda):
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_streams_side_by_side(cuda):
+    """Products of every launch form, the decode head and the scoring head on two streams at once: each takes
+    whole SMs, none waits for another's, and every result is what it is alone."""
+    sizes = [(5, 2560, 2560), (300, 4096, 1280), (64, 640, 2560), (700, 2560, 512)]
+    ops = [operands(*s, cuda, seed=i) for i, s in enumerate(sizes)]
+    w = (torch.randn(4096, 512, device=cuda) * 0.05).bfloat16()
+    hq, hs = P.fp8_target_lmhead.pack_fp8_block(w)
+    x = torch.randn(40, 512, device=cuda).bfloat16()
+    ids = torch.arange(300, device=cuda)
+
+    def everything():
+        out = [G.fp8_block_gemm(*o, out_dtype=torch.float32) for o in ops]
+        out += list(P.logprobs.fp8_head_logprobs(*ops[1], ids))
+        return out + list(P.fp8_target_lmhead.fp8_lmhead(x, hq, hs)[1:])
+
+    alone = everything()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = [[], []]
+    for _ in range(20):
+        for s, r in zip(streams, results):
+            with torch.cuda.stream(s):
+                r.append(everything())
+    torch.cuda.synchronize()
+    for r in results:
+        for got in r:
+            assert all(torch.equal(u, v) for u, v in zip(alone, got))
+    assert P._lib.score().b200_score_error(1) == 0
+
+
+@pytest.mark.parametrize("M,N,K", [(33, 136, 20480), (200, 520, 16400)])
+def test_long_k(cuda, M, N, K):
+    ops = operands(M, N, K, cuda, seed=K)
+    check(G.fp8_block_gemm(*ops, out_dtype=torch.float32), *ops)
