@@ -683,6 +683,55 @@ int num_sms() {
   return cached[dev];
 }
 
+// Raises the kernel's shared-memory limit, once per device, and checks what its register split relies on.
+template <int CG, int BN, int OUT>
+int make_ready(int dev) {
+  static bool ready[MAX_DEVICES] = {};
+  if (dev < MAX_DEVICES && ready[dev]) return 0;
+  const void* kern = reinterpret_cast<const void*>(product_kernel<CG, BN, OUT>);
+  if (Tile<BN>::SPLIT_REGS) {                         // the split's sum must be what the launch brings
+    cudaFuncAttributes fa;
+    const cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+    if (e != cudaSuccess) return (int)e;
+    if (fa.numRegs != Tile<BN>::LAUNCH_REGS) return -13;
+  }
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_CAP);
+  if (e == cudaSuccess && dev < MAX_DEVICES) ready[dev] = true;
+  return (int)e;
+}
+
+// How many clusters of `split` CTAs the device holds at once (fewer than its SMs / split: a cluster stays within a
+// group of SMs), asked once per device.
+template <int BN, int OUT>
+int clusters_at_once(int split) {
+  static int cached[MAX_DEVICES][4] = {};
+  const int at = split == 2 ? 1 : split == 4 ? 2 : split == 8 ? 3 : 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= MAX_DEVICES) return num_sms() / split * 3 / 4;
+  if (cached[dev][at] > 0) return cached[dev][at];
+  int n = 0;
+  if (split == 1) {
+    n = num_sms();
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(num_sms() / split * split);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = SMEM_MIN;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = split;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (make_ready<1, BN, OUT>(dev) != 0 ||
+        cudaOccupancyMaxActiveClusters(&n, product_kernel<1, BN, OUT>, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();                             // the launch itself will say what is wrong
+      return num_sms() / split * 3 / 4;
+    }
+  }
+  return cached[dev][at] = n;
+}
+
 template <int CG, int BN, int OUT>
 int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   constexpr int B_ROWS = BN / CG;
@@ -714,21 +763,11 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   p.nstage = std::min({MAX_STAGES, (SMEM_CAP - fixed) / stage, std::max(2, per_cta)});
   const int smem = std::max(SMEM_MIN, fixed + p.nstage * stage);
   auto kern = product_kernel<CG, BN, OUT>;
-  static bool ready[MAX_DEVICES] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return (int)e;
-  if (dev >= MAX_DEVICES || !ready[dev]) {
-    if (Tile<BN>::SPLIT_REGS) {                       // the split's sum must be what the launch brings
-      cudaFuncAttributes fa;
-      e = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(kern));
-      if (e != cudaSuccess) return (int)e;
-      if (fa.numRegs != Tile<BN>::LAUNCH_REGS) return -13;
-    }
-    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kern), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_CAP);
-    if (e != cudaSuccess) return (int)e;
-    if (dev < MAX_DEVICES) ready[dev] = true;
-  }
+  rc = make_ready<CG, BN, OUT>(dev);
+  if (rc != 0) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * cl);
   cfg.blockDim = dim3(THREADS);
@@ -753,7 +792,8 @@ int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
   // start, the busiest SM's 128-K blocks, and with K split the sums' way to their owners, in measured microseconds.
   // Measured there, chosen first: 5 x 2560 x 2560 at (128, 4) 7.2, (64, 2) 8.0, (64, 1) 9.7; 512 x 1024 x 2560 at
   // (64, 1) 9.7, (64, 2) 9.9, (128, 4) 12.2; 16 x 10240 x 2560 at (128, 1) 11.9, (64, 1) 16.6; 8192 x 10240 x 2560
-  // at 256 columns 201, (128, 1) 300.
+  // at 256 columns 201, (128, 1) 300. K is split only as far as all clusters run at once: counted by SMs alone,
+  // 1 x 1024 x 2560 and 64 x 1024 x 2560 took 8 CTAs a tile and a second turn, 9.8 and 12.0 for 6.1 and 7.4.
   const int KB = (o.K + 127) / 128, sms = num_sms();
   int bn = 256, split = 1;
   double best = 1e300;
@@ -768,10 +808,11 @@ int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
     consider(256, 1, (rows + 1) / 2 * ((o.N + 255) / 256), sms / 2, 5.0, 0.56);
   else
     consider(256, 1, (o.N + 255) / 256, sms, 5.0, 0.50);
-  for (int s = 1; OUT != OUT_STATS && s <= 8; s *= 2) {
-    consider(128, s, rows * ((o.N + 127) / 128) * s, sms, 4.6, 0.40);
-    consider(64, s, rows * ((o.N + 63) / 64) * s, sms, 3.6, 0.31);
-  }
+  if constexpr (OUT != OUT_STATS)
+    for (int s = 1; s <= 8; s *= 2) {
+      consider(128, s, rows * ((o.N + 127) / 128) * s, clusters_at_once<128, OUT>(s) * s, 4.6, 0.40);
+      consider(64, s, rows * ((o.N + 63) / 64) * s, clusters_at_once<64, OUT>(s) * s, 3.6, 0.31);
+    }
   if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, 1, stream) : launch<1, 256, OUT>(o, p, 1, stream);
   if constexpr (OUT != OUT_STATS)
     return bn == 128 ? launch<1, 128, OUT>(o, p, split, stream) : launch<1, 64, OUT>(o, p, split, stream);
