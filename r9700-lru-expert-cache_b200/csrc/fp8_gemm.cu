@@ -674,10 +674,10 @@ int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es
 
 constexpr int MAX_DEVICES = 64;
 
-int num_sms() {
+int num_sms(int dev) {
   static int cached[MAX_DEVICES] = {};
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= MAX_DEVICES) return 148;
+  int n = 0;
+  if (dev < 0 || dev >= MAX_DEVICES) return 148;
   if (cached[dev] <= 0)
     cached[dev] = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && n > 0 ? n : 148;
   return cached[dev];
@@ -703,37 +703,33 @@ int make_ready(int dev) {
 // How many clusters of `split` CTAs the device holds at once (fewer than its SMs / split: a cluster stays within a
 // group of SMs), asked once per device.
 template <int BN, int OUT>
-int clusters_at_once(int split) {
+int clusters_at_once(int dev, int split) {
   static int cached[MAX_DEVICES][4] = {};
-  const int at = split == 2 ? 1 : split == 4 ? 2 : split == 8 ? 3 : 0;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev >= MAX_DEVICES) return num_sms() / split * 3 / 4;
-  if (cached[dev][at] > 0) return cached[dev][at];
+  if (split == 1) return num_sms(dev);
+  const int at = split == 2 ? 1 : split == 4 ? 2 : 3;
+  if (dev < MAX_DEVICES && cached[dev][at] > 0) return cached[dev][at];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(num_sms(dev) / split * split);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = SMEM_MIN;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   int n = 0;
-  if (split == 1) {
-    n = num_sms();
-  } else {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(num_sms() / split * split);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = SMEM_MIN;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = split;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (make_ready<1, BN, OUT>(dev) != 0 ||
-        cudaOccupancyMaxActiveClusters(&n, product_kernel<1, BN, OUT>, &cfg) != cudaSuccess || n <= 0) {
-      cudaGetLastError();                             // the launch itself will say what is wrong
-      return num_sms() / split * 3 / 4;
-    }
+  if (make_ready<1, BN, OUT>(dev) != 0 ||
+      cudaOccupancyMaxActiveClusters(&n, product_kernel<1, BN, OUT>, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();                               // the launch itself will say what is wrong
+    return num_sms(dev) / split * 3 / 4;
   }
-  return cached[dev][at] = n;
+  if (dev < MAX_DEVICES) cached[dev][at] = n;
+  return n;
 }
 
 template <int CG, int BN, int OUT>
-int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
+int launch(const Operands& o, Product p, int dev, int split, cudaStream_t stream) {
   constexpr int B_ROWS = BN / CG;
   p.xs = o.xs, p.xs_row = o.xs_row, p.xs_col = o.xs_col, p.ws = o.ws, p.ws_row = o.ws_row;
   p.M = o.M, p.N = o.N, p.K = o.K, p.packed = o.packed;
@@ -751,7 +747,7 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   const int cl = CG == 2 ? 2 : split;
   // As few CTAs (pairs) as take no more turns than all SMs would: 8 x 151936 x 2560, whose 594 tiles are four turns and
   // two tiles of 148 SMs, takes 73 us on 119 and 76 on 148.
-  const int turns = split > 1 ? 1 : (tiles + num_sms() / cl - 1) / (num_sms() / cl);
+  const int turns = split > 1 ? 1 : (tiles + num_sms(dev) / cl - 1) / (num_sms(dev) / cl);
   const int clusters = (tiles + turns - 1) / turns;
   const int per_cta = split > 1 ? (KB + split - 1) / split : turns * KB;
   const bool few = CG == 1 && p.row_tiles == 1;
@@ -763,9 +759,6 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   p.nstage = std::min({MAX_STAGES, (SMEM_CAP - fixed) / stage, std::max(2, per_cta)});
   const int smem = std::max(SMEM_MIN, fixed + p.nstage * stage);
   auto kern = product_kernel<CG, BN, OUT>;
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) return (int)e;
   rc = make_ready<CG, BN, OUT>(dev);
   if (rc != 0) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -779,7 +772,7 @@ int launch(const Operands& o, Product p, int split, cudaStream_t stream) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kern, xmap, wmap, ymap, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, xmap, wmap, ymap, p);
   return (int)(e != cudaSuccess ? e : cudaGetLastError());
 }
 
@@ -794,7 +787,10 @@ int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
   // (64, 1) 9.7, (64, 2) 9.9, (128, 4) 12.2; 16 x 10240 x 2560 at (128, 1) 11.9, (64, 1) 16.6; 8192 x 10240 x 2560
   // at 256 columns 201, (128, 1) 300. K is split only as far as all clusters run at once: counted by SMs alone,
   // 1 x 1024 x 2560 and 64 x 1024 x 2560 took 8 CTAs a tile and a second turn, 9.8 and 12.0 for 6.1 and 7.4.
-  const int KB = (o.K + 127) / 128, sms = num_sms();
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  const int KB = (o.K + 127) / 128, sms = num_sms(dev);
   int bn = 256, split = 1;
   double best = 1e300;
   auto consider = [&](int b, int s, long long ctas, int at_once, double start, double block) {
@@ -810,12 +806,12 @@ int launch_product(const Operands& o, const Product& p, cudaStream_t stream) {
     consider(256, 1, (o.N + 255) / 256, sms, 5.0, 0.50);
   if constexpr (OUT != OUT_STATS)
     for (int s = 1; s <= 8; s *= 2) {
-      consider(128, s, rows * ((o.N + 127) / 128) * s, clusters_at_once<128, OUT>(s) * s, 4.6, 0.40);
-      consider(64, s, rows * ((o.N + 63) / 64) * s, clusters_at_once<64, OUT>(s) * s, 3.6, 0.31);
+      consider(128, s, rows * ((o.N + 127) / 128) * s, clusters_at_once<128, OUT>(dev, s) * s, 4.6, 0.40);
+      consider(64, s, rows * ((o.N + 63) / 64) * s, clusters_at_once<64, OUT>(dev, s) * s, 3.6, 0.31);
     }
-  if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, 1, stream) : launch<1, 256, OUT>(o, p, 1, stream);
+  if (bn == 256) return o.M > BM ? launch<2, 256, OUT>(o, p, dev, 1, stream) : launch<1, 256, OUT>(o, p, dev, 1, stream);
   if constexpr (OUT != OUT_STATS)
-    return bn == 128 ? launch<1, 128, OUT>(o, p, split, stream) : launch<1, 64, OUT>(o, p, split, stream);
+    return bn == 128 ? launch<1, 128, OUT>(o, p, dev, split, stream) : launch<1, 64, OUT>(o, p, dev, split, stream);
   return -8;
 }
 
