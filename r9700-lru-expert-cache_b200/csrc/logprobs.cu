@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
         ref = moved;
         limit = top + HEADROOM / LOG2E;
       }
-      if (top > xt) {
+      if (!(top <= xt)) {                                    // (top is NaN where the chunk holds one: its others count)
         if constexpr (C::PACKED) {
           auto count = C::both(0.f);
           const auto t2 = C::both(xt);
