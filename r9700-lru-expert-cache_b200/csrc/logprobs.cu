@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) token_logprobs_kernel
           for (int j = 0; j < N; ++j) {
             const long long e = (long long)c * N - shift + j;
             const unsigned long long key = e >= 0 && e < V ? order_key(C::value(v, j), (int)e) : 0;
-            if (key < last) best = max(best, key);
+            if (t == 0 || key < last) best = max(best, key);    // (NaN at id 0 has the largest key there is)
           }
         }
 #pragma unroll

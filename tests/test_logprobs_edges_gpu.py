@@ -44,3 +44,14 @@ def test_rank_beside_nan(cuda, dtype, V, off):
     assert r.rank[4] == 1
     for t in (r.logprob, r.entropy, r.logsumexp):
         assert torch.isnan(t).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,V,k", [(1, 64, 64), (2, 9001, 20), (200, 151936, 64)])
+def test_top_of_rows_of_nothing_but_nan(cuda, dtype, M, V, k):
+    """NaN comes first and equal ones by the lower id: 0, 1, 2 ... where every logit is NaN, also in a CTA
+    that has a whole long row and so more of them than it keeps."""
+    x = torch.full((M, V), math.nan, dtype=dtype, device=cuda)
+    r = LP.token_logprobs(x, torch.zeros(M, dtype=torch.int64, device=cuda), top_k=k)
+    assert torch.equal(r.top_ids, torch.arange(k, device=cuda).expand(M, k))
+    assert torch.isnan(r.top_logprobs).all() and (r.rank == 1).all()
