@@ -52,8 +52,10 @@ int b200_fp8_head_logprobs(const void* qx, long long ldx, const float* xs, long 
                            const long long* ids, int M, int N, int K, float* logprob, float* entropy, float* lse,
                            void* workspace, long long workspace_bytes, cudaStream_t stream);
 
-/* Device error word of these kernels (1 = a bounded pipeline wait ran out, and that call's outputs are
- * not complete); reset != 0 clears it. Synchronous. */
+/* Device error word of these kernels (1 = a bounded pipeline wait ran out: what that call could not compute
+ * is NaN, an element of the product or a row's logprob, entropy and lse); reset != 0 clears it. Synchronous
+ * with the default stream: synchronize any other stream first. A wait gives up after 2^18 tries, about a
+ * second, or as many as B200_SCORE_WAIT_TRIES in the environment says at the first call (0: at once). */
 int b200_score_error(int reset);
 
 #ifdef __cplusplus

@@ -173,7 +173,8 @@ def debug_check(what: str) -> None:
 
 
 def debug_check_score(what: str) -> None:
-    """debug_check for the scoring kernels' own error word."""
+    """debug_check for the scoring kernels' own error word. (Without it such a call's product is NaN
+    where it is not complete, and so are the log probabilities, entropy and logsumexp of such rows.)"""
     if not _CHECK:
         return
     import torch

@@ -21,6 +21,7 @@
 // four accumulators in flight; and the chip's power, which holds the clock near 1.6 GHz. The tensor pipe is active
 // 59 % of the time. Few tokens stream the weight: 8 x 151936 x 2560 takes 67 us, 5.8 TB/s.
 #include <algorithm>
+#include <cstdlib>
 
 #include <cudaTypedefs.h>
 
@@ -61,11 +62,13 @@ struct Product {
   void* y;
   long long ldy;
   int tma_out;                             // y's base and rows are 16-byte aligned
+  uint32_t tries;                          // of a pipeline wait before it gives up
   // head: of every row and column tile {m, s, w, 0}; of every row its token's logit
   const long long* ids;
   float4* part;
   float* token;
 };
+static_assert(sizeof(Product) <= 128, "one word more and the 256-column tiles spill 120 bytes a thread");
 
 enum Out { OUT_BF16 = 0, OUT_F16 = 1, OUT_F32 = 2, OUT_STATS = 3 };
 
@@ -350,17 +353,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       // ---------------- copies ----------------
       bool ok = true;
       while (at.t < tiles && ok) {
-        ok = at.round == 0 || mbar_wait_limited(&empty[at.s], (at.round - 1) & 1);
+        ok = at.round == 0 || mbar_wait_limited(&empty[at.s], (at.round - 1) & 1, p.tries);
         if (ok) copy_next();
       }
       // Leave only when this CTA's copies have landed and been read: the MMAs' commit of each stage's last use.
       const long long oldest = at.count > nstage ? at.count - nstage : 0;
       for (long long q = oldest; q < at.count && ok; ++q)
-        ok = mbar_wait_limited(&empty[q % nstage], (uint32_t)(q / nstage) & 1);
+        ok = mbar_wait_limited(&empty[q % nstage], (uint32_t)(q / nstage) & 1, p.tries);
       if (!ok) {
         atomicExch(&g_score_err, 1);
         if (CG == 1 || rank == 0)
-          for (long long q = oldest; q < at.count; ++q) mbar_wait_limited(&full[q % nstage], (uint32_t)(q / nstage) & 1);
+          for (long long q = oldest; q < at.count; ++q)
+            mbar_wait_limited(&full[q % nstage], (uint32_t)(q / nstage) & 1, WAIT_TRIES);
         else                                           // the pair's barriers are the other CTA's: time for any copy to land
           for (const uint64_t t0 = globaltimer_ns(); globaltimer_ns() - t0 < 10000000ull;) __nanosleep(1000);
       }
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (s >= nstage) s -= nstage, ++round;
       bool ok = true;
       for (long long i = UNITS == 2 ? 0 : u; i < blocks; i += STEP) {
-        ok = warp_wait(&full[s], round & 1, &acc_empty[buf], (use - 1) & 1, use > 0);
+        ok = warp_wait(&full[s], round & 1, &acc_empty[buf], (use - 1) & 1, use > 0, p.tries);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
@@ -407,7 +411,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_commit<CG>(&done[u]);
         }
         __syncwarp();
-        mbar_wait_limited(&done[u], 0);
+        mbar_wait_limited(&done[u], 0, WAIT_TRIES);
       }
     }
     __syncwarp();
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int j = 0; j < BM / 8; ++j)
           x[j] = kb + i < kb1 && m + 8 * j < p.M
                      ? __ldg(p.xs + (long long)(m + 8 * j) * p.xs_row + (long long)(kb + i) * p.xs_col) : 0.f;
-        if (fg >= 2) ok = warp_wait(&f_empty[fg & 1], ((fg >> 1) - 1) & 1);
+        if (fg >= 2) ok = warp_wait(&f_empty[fg & 1], ((fg >> 1) - 1) & 1, p.tries);
         if (!ok) break;
         float* dst = factors + ((fg & 1) * FGROUP + i) * F_LD + r8;
 #pragma unroll
@@ -461,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int c = 0; c < W / 2; ++c) acc[c] = make_float2(0.f, 0.f);
       for (int kb = kb0; kb < kb1 && ok; ++kb) {
         const int fi = (kb - kb0) & (FGROUP - 1);
-        ok = warp_wait(&acc_full[buf], use & 1, &f_full[fg & 1], (fg >> 1) & 1, fi == 0);
+        ok = warp_wait(&acc_full[buf], use & 1, &f_full[fg & 1], (fg >> 1) & 1, fi == 0, p.tries);
         if (!ok) break;
         tc_fence_after();
         const float* now = my_factors + ((fg & 1) * FGROUP + fi) * F_LD;
@@ -489,11 +493,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         buf += UNITS;
         if (buf >= NBUF) buf -= NBUF, ++use;
       }
+      if (!ok) {                                       // a wait ran out: this tile and the rest come out NaN
+#pragma unroll
+        for (int c = 0; c < W / 2; ++c) acc[c] = make_float2(NAN, NAN);
+      }
       if constexpr (OUT == OUT_STATS) {
         // a tile's four column groups leave one set of statistics
         float* own = stat_s + (turn & 1) * 3 * EPI_GROUPS * BM + row_in_tile;
         LogitStat st = logit_stat_empty();
-        if (ok && m < p.M && n < p.N) st = row_stats<W, SEG>(p, m, n, acc);
+        if (m < p.M && n < p.N) st = row_stats<W, SEG>(p, m, n, acc);
         own[(0 * EPI_GROUPS + group) * BM] = st.m;
         own[(1 * EPI_GROUPS + group) * BM] = st.s;
         own[(2 * EPI_GROUPS + group) * BM] = st.w;
@@ -505,7 +513,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           p.part[(long long)m * p.col_tiles + ct] = make_float4(st.m, st.s, st.w, 0.f);
         }
         ++turn;
-      } else if (ok && split == 1 && n < p.N && m - lane < p.M) {
+      } else if (split == 1 && n < p.N && m - lane < p.M) {
         store_rows<OUT, W, SEG>(p, &ymap, sm + out_offset() + (group * quarters + quarter) * OUT_BUFS * OUT_BUF, turn,
                                 m - lane, n, lane, acc);
       }
@@ -672,6 +680,15 @@ int out_map(CUtensorMap* m, void* base, int rows, int cols, long long ld, int es
             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -12;
 }
 
+// Tries of a pipeline wait: WAIT_TRIES, or what the environment says when the first call is made.
+uint32_t wait_tries() {
+  static const uint32_t n = [] {
+    const char* s = std::getenv("B200_SCORE_WAIT_TRIES");
+    return s != nullptr && *s >= '0' && *s <= '9' ? (uint32_t)std::strtoul(s, nullptr, 10) : WAIT_TRIES;
+  }();
+  return n;
+}
+
 constexpr int MAX_DEVICES = 64;
 
 int num_sms(int dev) {
@@ -733,6 +750,7 @@ int launch(const Operands& o, Product p, int dev, int split, cudaStream_t stream
   constexpr int B_ROWS = BN / CG;
   p.xs = o.xs, p.xs_row = o.xs_row, p.xs_col = o.xs_col, p.ws = o.ws, p.ws_row = o.ws_row;
   p.M = o.M, p.N = o.N, p.K = o.K, p.packed = o.packed;
+  p.tries = wait_tries();
   p.box_m = std::min(BM, (o.M + 7) / 8 * 8);
   p.row_tiles = (o.M + BM * CG - 1) / (BM * CG);
   p.col_tiles = (o.N + BN - 1) / BN;

@@ -148,8 +148,9 @@ B200_DEVINL void st_cluster_f4(uint32_t cluster_addr, float4 v) {
 // need two barriers wait for both at once, on different lanes.
 
 constexpr uint32_t WAIT_TRIES = 1u << 18;            // about a second
-// Waits for a phase. false: it did not come, and the caller records an error and leaves.
-B200_DEVINL bool mbar_wait_limited(uint64_t* bar, uint32_t parity) {
+// Waits for a phase, with `tries` tries. false: it did not come (or tries is 0), and the caller records an error and
+// leaves.
+B200_DEVINL bool mbar_wait_limited(uint64_t* bar, uint32_t parity, uint32_t tries) {
   uint32_t ok;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\tmov.u32 n, 0;\n"
@@ -157,20 +158,21 @@ B200_DEVINL bool mbar_wait_limited(uint64_t* bar, uint32_t parity) {
       "add.u32 n, n, 1;\n\tsetp.lt.u32 q, n, %3;\n\t@q bra TRY_%=;\n"
       "DONE_%=:\n\tselp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "n"(WAIT_TRIES)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(tries)
       : "memory");
-  return ok != 0;
+  return ok != 0 && tries != 0;
 }
 // The warp waits for `bar` and, where `both`, for `other` too. Uniform. What either barrier guards is there for
 // every lane, although each lane waited for one of them: the vote alone would let a load be moved ahead of it.
-B200_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t* other, uint32_t other_parity, bool both) {
+B200_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, uint64_t* other, uint32_t other_parity, bool both,
+                           uint32_t tries) {
   const bool second = both && (lane_id() & 1);
-  const bool ok = __all_sync(0xffffffffu, mbar_wait_limited(second ? other : bar, second ? other_parity : parity));
+  const bool ok = __all_sync(0xffffffffu, mbar_wait_limited(second ? other : bar, second ? other_parity : parity, tries));
   __syncwarp();
   return ok;
 }
-B200_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity) {
-  return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity));
+B200_DEVINL bool warp_wait(uint64_t* bar, uint32_t parity, uint32_t tries) {
+  return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, tries));
 }
 
 // ---- tensor-map copies -------------------------------------------------------------------------
