@@ -99,9 +99,15 @@ def score_prompt(hidden: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, token
     token_ids[i]) quantized per group of 128, through the FP8 head (wq, ws), the strip pack of
     ``pack_fp8_block`` by default. Without alternatives (top_k 0) the logits are never written;
     with them they are, as bf16, for ``rows_at_once`` rows at a time."""
-    from .fused_silu_mul_quant import per_token_group_quant_fp8
     if rows_at_once < 1:
         raise ValueError("score_prompt: rows_at_once must be at least 1")
+    _lib.require_cuda("score_prompt", hidden)
+    with torch.cuda.device(hidden.device):           # (the quantiser launches on the current device)
+        return _score_prompt(hidden, wq, ws, token_ids, top_k, packed, rows_at_once)
+
+
+def _score_prompt(hidden, wq, ws, token_ids, top_k, packed, rows_at_once):
+    from .fused_silu_mul_quant import per_token_group_quant_fp8
     qx, xs = per_token_group_quant_fp8(hidden)
     if top_k == 0:
         return fp8_head_logprobs(qx, wq, xs, ws, token_ids, packed=packed)
