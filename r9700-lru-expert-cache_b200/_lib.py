@@ -139,11 +139,10 @@ def launch(what: str, fn, device, *args) -> None:
     code. (The raw stream handle: building a torch.cuda.Stream for it costs as much as the launch.)"""
     import torch
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
+    if index != torch._C._cuda_getDevice():
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            return launch(what, fn, device, *args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         check(rc, what)
     if _CHECK:
@@ -173,8 +172,9 @@ def debug_check(what: str) -> None:
 
 
 def debug_check_score(what: str) -> None:
-    """debug_check for the scoring kernels' own error word. (Without it such a call's product is NaN
-    where it is not complete, and so are the log probabilities, entropy and logsumexp of such rows.)"""
+    """debug_check for the scoring kernels' own error word, on the current device. (Without it such a
+    call's product is NaN where it is not complete, and so are the log probabilities, entropy and
+    logsumexp of such rows.)"""
     if not _CHECK:
         return
     import torch

@@ -66,3 +66,24 @@ def test_score_prompt_runs_on_its_tensors_device(monkeypatch, current, top_k):
 def test_score_prompt_refuses_host_tensors():
     with pytest.raises(ValueError, match="CUDA"):
         LP.score_prompt(torch.zeros(2, 128), torch.zeros(16, 128), torch.zeros(1, 1), torch.zeros(2, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_debug_check_looks_at_the_launch_device(monkeypatch, current, index):
+    """With B200_LMHEAD_CHECK=1 a call waits for its own device's stream and reads that device's error word."""
+    seen = []
+
+    def note(name, result):
+        return lambda *a: (seen.append((name, current.now)), result)[1]
+
+    stream = types.SimpleNamespace(synchronize=note("wait", None))
+    lib = types.SimpleNamespace(b200_score_error=note("word", 0))
+    monkeypatch.setattr(P._lib, "_CHECK", True)
+    monkeypatch.setattr(P._lib, "score", lambda: lib)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: stream)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current.now, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 100 + i, raising=False)
+    P._lib.launch("call", lambda *a: (seen.append(("launch", current.now)), seen.append(a))[0] or 0,
+                  torch.device("cuda", index), 7)
+    assert seen == [("launch", index), (7, 100 + index), ("wait", index), ("word", index)]
+    assert current.now == 0
