@@ -55,3 +55,40 @@ def test_top_of_rows_of_nothing_but_nan(cuda, dtype, M, V, k):
     r = LP.token_logprobs(x, torch.zeros(M, dtype=torch.int64, device=cuda), top_k=k)
     assert torch.equal(r.top_ids, torch.arange(k, device=cuda).expand(M, k))
     assert torch.isnan(r.top_logprobs).all() and (r.rank == 1).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,V", [(1, 151936), (9, 151936), (512, 151936), (40, 5003)])
+@pytest.mark.parametrize("peak", [12.0, 20.0, 30.0, 39.0, 60.0])
+def test_peaked_rows(cuda, dtype, M, V, peak):
+    """One logit far above the others, as in most rows of a text: nothing is lost against sums relative to
+    the row's maximum, no log probability is above 0 and no entropy below.
+
+    Tolerance, with t = 1 - p_max and W = sum p d (d = x - max). Relative to the maximum its term is 1 to
+    exp2's 2^-22, the others together t with 2^-22 + 50 2^-24 for each term's argument and at most 600
+    2^-24 for a thread's additions; the additions to the maximum's own sum lose no more than what is added
+    (t), and no more than 300 of 2^-24; 16 further operations of 2^-24 join threads, warps and CTAs. So
+    ln S is off by a = 2^-22 + 16 2^-24 + t 2^-14 + min(t, 300 2^-24), the entropy by a + |W| 2^-14 and
+    the results' own rounding (three operations) is 2^-22 of their size."""
+    x, ids = logits(M, V, dtype, cuda, seed=int(peak), scale=2.5)
+    at = torch.randint(V, (M,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(M))
+    x[torch.arange(M, device=cuda), at] = peak
+    ids[::3] = at[::3]
+    p = torch.log_softmax(x.double(), 1)
+    prob = torch.exp(p)
+    others = prob.clone()
+    others.scatter_(1, x.argmax(1, keepdim=True), 0.0)
+    t = others.sum(1)
+    d = x.double() - x.amax(1, keepdim=True).double()
+    mean = (prob * d).sum(1).abs()
+    a = 2.0 ** -22 + 16 * 2.0 ** -24 + t * 2.0 ** -14 + t.clamp(max=300 * 2.0 ** -24)
+    r = LP.token_logprobs(x, ids, top_k=3)
+    want = p.gather(1, ids[:, None])[:, 0]
+    assert ((r.logprob - want).abs() <= a + 2.0 ** -22 * want.abs()).all()
+    lse = torch.logsumexp(x.double(), 1)
+    assert ((r.logsumexp - lse).abs() <= a + 2.0 ** -22 * lse.abs()).all()
+    entropy = -(prob * p).sum(1)
+    assert ((r.entropy - entropy).abs() <= a + mean * 2.0 ** -14 + 2.0 ** -22 * entropy).all()
+    top = p.gather(1, r.top_ids)
+    assert ((r.top_logprobs - top).abs() <= a[:, None] + 2.0 ** -22 * top.abs()).all()
+    assert (r.logprob <= 0).all() and (r.top_logprobs <= 0).all() and (r.entropy >= 0).all()
