@@ -90,8 +90,8 @@ B200_DEVINL RowResult logit_stat_finish(const LogitStat& st, float xt, bool vali
   } else {
     const float ls = logf(st.s);
     r.lse = st.m + ls;
-    r.entropy = ls - st.w / st.s;
-    r.logprob = (xt - st.m) - ls;
+    r.entropy = fmaxf(ls - st.w / st.s, 0.f);        // (a sum a rounding below 1 has a logarithm below 0)
+    r.logprob = fminf((xt - st.m) - ls, 0.f);
   }
   if (isnan(st.s)) r.lse = r.entropy = r.logprob = NAN;
   if (!valid) r.logprob = NAN;

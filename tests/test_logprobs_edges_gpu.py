@@ -92,3 +92,17 @@ def test_peaked_rows(cuda, dtype, M, V, peak):
     top = p.gather(1, r.top_ids)
     assert ((r.top_logprobs - top).abs() <= a[:, None] + 2.0 ** -22 * top.abs()).all()
     assert (r.logprob <= 0).all() and (r.top_logprobs <= 0).all() and (r.entropy >= 0).all()
+
+
+@pytest.mark.parametrize("M", [4, 128, 300])
+@pytest.mark.parametrize("scale", [1.0, 30.0, 100.0, 1000.0])
+def test_head_signs(cuda, M, scale):
+    """The head's log probabilities are never above 0 and its entropies never below, however sharp a row
+    is: exactly, since text is mostly rows whose largest logit has all of the probability."""
+    from test_fp8_block_gemm_gpu import operands, reference
+    qx, wq, xs, ws = operands(M, 5000, 512, cuda, seed=3)
+    xs *= scale
+    y, _ = reference(qx, wq, xs, ws)
+    r = LP.fp8_head_logprobs(qx, wq, xs, ws, y.argmax(1))
+    assert (r.logprob <= 0).all() and (r.entropy >= 0).all()
+    assert (r.logsumexp >= y.amax(1).float() * (1 - 1e-5) - 1e-4).all()
