@@ -98,7 +98,8 @@ def score_prompt(hidden: torch.Tensor, wq: torch.Tensor, ws: torch.Tensor, token
     """The log probabilities of a prompt's tokens: hidden bf16 or f16 [M, K] (row i predicts
     token_ids[i]) quantized per group of 128, through the FP8 head (wq, ws), the strip pack of
     ``pack_fp8_block`` by default. Without alternatives (top_k 0) the logits are never written;
-    with them they are, as bf16, for ``rows_at_once`` rows at a time."""
+    with them they are, in 32 bits like the head's own, for ``rows_at_once`` rows at a time (4 bytes a
+    row and token of the vocabulary)."""
     if rows_at_once < 1:
         raise ValueError("score_prompt: rows_at_once must be at least 1")
     _lib.require_cuda("score_prompt", hidden)
@@ -114,7 +115,7 @@ def _score_prompt(hidden, wq, ws, token_ids, top_k, packed, rows_at_once):
     M = hidden.shape[0]
     ids = _ids("score_prompt", token_ids, M, hidden.device)
     parts = []
-    logits = torch.empty(min(M, rows_at_once), wq.shape[0], dtype=torch.bfloat16, device=hidden.device)
+    logits = torch.empty(min(M, rows_at_once), wq.shape[0], dtype=torch.float32, device=hidden.device)
     for r0 in range(0, max(M, 1), rows_at_once):
         r1 = min(M, r0 + rows_at_once)
         y = fp8_block_gemm(qx[r0:r1], wq, xs[r0:r1], ws, out=logits[:r1 - r0], packed=packed)

@@ -106,3 +106,29 @@ def test_head_signs(cuda, M, scale):
     r = LP.fp8_head_logprobs(qx, wq, xs, ws, y.argmax(1))
     assert (r.logprob <= 0).all() and (r.entropy >= 0).all()
     assert (r.logsumexp >= y.amax(1).float() * (1 - 1e-5) - 1e-4).all()
+
+
+@pytest.mark.parametrize("M,rows", [(1, 1024), (70, 32), (300, 1024)])
+def test_alternatives_do_not_change_a_score(cuda, M, rows):
+    """score_prompt with alternatives and without: both from the product in 32 bits, so both within what
+    the head's own test allows (2e-4), the rank and the alternatives exactly those of that product."""
+    N, K = 5120, 512
+    g = torch.Generator(device=cuda).manual_seed(M + 1)
+    hidden = torch.randn(M, K, device=cuda, generator=g).bfloat16()
+    w = (torch.randn(N, K, device=cuda, generator=g) * 0.2).bfloat16()
+    ids = torch.randint(N, (M,), device=cuda, generator=g)
+    wq, ws = P.fp8_target_lmhead.pack_fp8_block(w)
+    a = LP.score_prompt(hidden, wq, ws, ids)
+    b = LP.score_prompt(hidden, wq, ws, ids, top_k=6, rows_at_once=rows)
+    qx, xs = P.fused_silu_mul_quant.per_token_group_quant_fp8(hidden)
+    y = torch.cat([P.fp8_block_gemm.fp8_block_gemm(qx[i:i + rows], wq, xs[i:i + rows], ws, out_dtype=torch.float32,
+                                                   packed=True) for i in range(0, M, rows)])
+    want = torch.log_softmax(y.double(), 1)
+    at = want.gather(1, ids[:, None])[:, 0]
+    for r in (a, b):
+        assert (r.logprob - at).abs().max() <= 2e-4
+        assert (r.entropy + (want.exp() * want).sum(1)).abs().max() <= 2e-4 * (1 + y.abs().max().item())
+        assert (r.logsumexp - torch.logsumexp(y.double(), 1)).abs().max() <= 2e-4
+    assert torch.equal(b.rank, 1 + (y > y.gather(1, ids[:, None])).sum(1))
+    assert torch.equal(b.top_ids, torch.sort(y, dim=1, descending=True, stable=True).indices[:, :6])
+    assert (b.top_logprobs - want.gather(1, b.top_ids)).abs().max() <= 2e-4
