@@ -22,9 +22,9 @@ extern "C" {
  * layout of b200_lmhead.h (N % 16 == 0, K % 128 == 0, ldw unused). y [M, N] with row stride ldy
  * elements. K % 16 == 0, ldx and ldw multiples of 16, 16-byte aligned qx and wq (a TMA copy's rules);
  * a last group of fewer than 128 K and a last block of fewer than 128 rows have scales of their own.
- * Returns 0, -1 M outside [0, 2^30], -2 bad N (at most 2^30), -3 bad K, -4 a stride below its row length or not a
- * multiple of 16, -5 bad dtype, -8 more than 2^30 tiles, -10 misaligned pointer, -12 no tensor map, -13 a build
- * whose register count is not the one the kernels were written for. */
+ * Returns 0, -1 M outside [0, 2^30], -2 bad N (at most 2^30), -3 bad K (at most 2^30), -4 a stride below its
+ * row length or not a multiple of 16, -5 bad dtype, -8 more than 2^30 tiles, -10 misaligned pointer, -12 no
+ * tensor map, -13 a build whose register count is not the one the kernels were written for. */
 int b200_fp8_block_gemm(const void* qx, long long ldx, const float* xs, long long xs_row, long long xs_col,
                         const void* wq, long long ldw, int packed, const float* ws, long long ws_row, void* y,
                         long long ldy, int y_dtype, int M, int N, int K, cudaStream_t stream);

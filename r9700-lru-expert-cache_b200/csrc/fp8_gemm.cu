@@ -626,7 +626,7 @@ bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n =
 int check_operands(const Operands& p) {
   if (p.M < 0 || p.M > (1 << 30)) return -1;         // (coordinates and tile numbers are 32-bit)
   if (p.N < 1 || p.N > (1 << 30) || (p.packed && p.N % 16)) return -2;
-  if (p.K < 16 || p.K % 16 || (p.packed && p.K % 128)) return -3;
+  if (p.K < 16 || p.K > (1 << 30) || p.K % 16 || (p.packed && p.K % 128)) return -3;
   if (p.ldx < p.K || p.ldx % 16 || (!p.packed && (p.ldw < p.K || p.ldw % 16))) return -4;
   if (!aligned(p.x, 16) || !aligned(p.w, 16)) return -10;
   return 0;
