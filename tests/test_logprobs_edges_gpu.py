@@ -132,3 +132,36 @@ def test_alternatives_do_not_change_a_score(cuda, M, rows):
     assert torch.equal(b.rank, 1 + (y > y.gather(1, ids[:, None])).sum(1))
     assert torch.equal(b.top_ids, torch.sort(y, dim=1, descending=True, stable=True).indices[:, :6])
     assert (b.top_logprobs - want.gather(1, b.top_ids)).abs().max() <= 2e-4
+
+
+@pytest.mark.parametrize("M", [3, 300])
+def test_inside_a_graph_on_new_inputs(cuda, M):
+    """Both log probability calls captured in one CUDA graph (the head's merge is a programmatic dependent
+    of its product) and replayed after their inputs have changed: what the calls give outside it."""
+    from test_fp8_block_gemm_gpu import operands
+    qx, wq, xs, ws = operands(M, 5000, 512, cuda, seed=1)
+    x, ids = logits(M, 20000, torch.bfloat16, cuda, seed=1)
+    ids = ids % 5000
+
+    def both():
+        return [*LP.token_logprobs(x, ids, top_k=5), *LP.fp8_head_logprobs(qx, wq, xs, ws, ids)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        both()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = both()
+    for seed in (2, 3):
+        for old, new in zip((qx, wq, xs, ws), operands(M, 5000, 512, cuda, seed=seed)):
+            old.copy_(new)
+        x.copy_(logits(M, 20000, torch.bfloat16, cuda, seed=seed)[0])
+        ids.copy_((ids + 1) % 5000)
+        for t in got:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(got, both()):
+            assert torch.equal(u, v)
