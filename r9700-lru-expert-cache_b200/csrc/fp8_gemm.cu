@@ -15,11 +15,14 @@
 // CTAs (or pairs) walk the tiles, rows first within groups of row tiles, so that tiles in flight share weights.
 //
 // Above 128 rows two CTAs share a tile of 256 rows x 256 columns (cta_group::2): a stage is 32 KB a CTA instead of
-// 48, which the L2 and the shared memory feel. What bounds it (8192 x 10240 x 2560, 201 us, 2130 TFLOP/s; one CTA
-// 216 us): a block's MMAs take 512 clocks, but its accumulators come free only after commit, two waits of 110 to 160
-// clocks, eight TMEM loads with their 64 multiply-adds, and the release to the issuing CTA, about 850 clocks with
-// four accumulators in flight; and the chip's power, which holds the clock near 1.6 GHz. The tensor pipe is active
-// 59 % of the time. Few tokens stream the weight: 8 x 151936 x 2560 takes 67 us, 5.8 TB/s.
+// 48, which the L2 and the shared memory feel (8192 x 10240 x 2560 201 us, one CTA 216). What bounds it: at a fixed
+// number of tiles and K from 512 to 10240 a block takes 830 to 870 clocks, 512 of them its MMAs (the tensor pipe is
+// active 59 % of the time), and a tile 2400 more. DRAM (11 %), L2 (34 %) and issue slots (48 %) are not full; which
+// part of an accumulator's way from commit through two waits (110 to 160 clocks each), eight TMEM loads with their 64
+// multiply-adds and release to the issuing CTA makes the difference has not been told apart. A tile of the head costs
+// about 7000 clocks beside its blocks, statistics that the MMAs do not hide. And the power limit: the product takes 200
+// to 209 us in a burst of some milliseconds (up to 2150 TFLOP/s), 240 once the clock has settled, at 1470 MHz. Few
+// tokens stream the weight: 8 x 151936 x 2560 takes 67 us, 5.8 TB/s.
 #include <algorithm>
 #include <cstdlib>
 

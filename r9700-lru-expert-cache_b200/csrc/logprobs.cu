@@ -19,10 +19,13 @@
 //
 // A row is shared by a cluster of 1 to 8 CTAs, so that few rows still occupy the SMs.
 //
-// What bounds it: without alternatives the row's bytes (4096 x 151936 bf16 in 209 us, 5.95 TB/s, 0.91 of a copy's
-// rate), at about seven instructions a logit, close behind the issue slots. With 20 alternatives 258 us: the second
-// reading, mostly from DRAM by then (27 KB of a row's 304), and seven barriers a row. Few rows: latency, 4.7 us for
-// one row, 8.4 with five alternatives. Against this layout: one exponent by subtraction and multiplication and a
+// What bounds it: without alternatives the row's bytes (4096 x 151936 bf16 in 205 us, 6.07 TB/s, 0.93 of a copy's
+// rate), at about seven instructions a logit, close behind the issue slots. With 20 alternatives 248 us: the second
+// reading, mostly from DRAM by then (27 KB of a row's 304), and seven barriers a row. Both in a burst of some
+// milliseconds: at the power limit, whose clock settles near 1.63 GHz, 243 and 288. Few rows: latency, 4.7 us for
+// one row, 8.4 with five alternatives. Rows with many logits equal to the bound are slow, since their chunks are all
+// read for it and overflow into the last resort, a pass for each alternative: a mask that leaves fewer tokens than
+// alternatives, or equal logits, took 14.6 ms at 4096 x 151936 with 20. Against this layout: one exponent by subtraction and multiplication and a
 // clamp per logit on 16-byte chunks took 292 and 378 us; CTAs of 512 threads 227 and 294, of 128 threads 207 and 494.
 #include <algorithm>
 
