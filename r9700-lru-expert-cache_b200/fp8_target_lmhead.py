@@ -252,7 +252,8 @@ class Fp8TargetHead:
 
     def score(self, hidden: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0):
         """The log probabilities of a prompt's tokens under this head (``logprobs.score_prompt``):
-        hidden [M, K] for any M, token_ids [M], with ``top_k`` alternatives of every row."""
+        hidden [M, K] for any M, token_ids [M], with ``top_k`` alternatives of every row. The softmax is
+        over this head's own rows: not for one shard of a vocabulary."""
         from .logprobs import score_prompt
         return score_prompt(hidden, self.wq, self.ws, token_ids, top_k=top_k)
 
